@@ -389,6 +389,142 @@ GPTOSS_API int gptoss_argmax_noalloc(gptoss_stream_t stream, int T, const void *
                                      gptoss_dtype_t logits_dtype, long V, long row_stride,
                                      int *out);
 
+/* ------------------------------------------------------------------------------------
+ * The 8-bit paged key/value cache: append, attention, pages.
+ *
+ * The reference has none of this (its cache has fixed slots per request, keys in bf16 and one
+ * scale per value vector, gptoss_kv_cache_write above).  A page holds 64 tokens.  For each page,
+ * key/value head and kind (0 key, 1 value) it has 64 x head_dim int8 codes and one fp32 scale
+ * that is a power of two; a value is code * scale, which is exact in bf16 and fp32.
+ *
+ * A sequence's token at position p lives in slot p % 64 of the page pages[s * pages_stride + p / 64]
+ * of its page table row; -1, or any number outside [0, n_pages), means that there is no page.  One
+ * table serves all layers of a pool.  Two sequences may share a page (gptoss_kv8_fork) as long as
+ * neither appends to it.
+ *
+ * A step's rows are rows of the rotated qkv tensor (gptoss_qkv_bias_rope's output), sequence after
+ * sequence: rows row_start[s] .. row_start[s + 1] - 1 (row_start has n_seqs + 1 entries, clamped
+ * into [0, T]) are the newest tokens of sequence s, whose length INCLUDING them is kv_len[s]; with q
+ * rows their positions are kv_len[s] - q .. kv_len[s] - 1.  A sequence without rows sits the step
+ * out.  max_new bounds the rows of any one sequence: rows of a sequence past its first max_new
+ * are not processed (1 for a decode step; T is always right).  row_start, kv_len and the table are
+ * device arrays that a captured graph reads afresh at every replay.
+ *
+ * head_dim is 64 or 128 and n_q_heads a multiple of n_kv_heads.  Results are the same at every run
+ * (no atomics whose order shows).  These entry points know GPTOSS_PDL; the arithmetic flags do not
+ * apply to them and are ignored.
+ */
+#define GPTOSS_KV8_PAGE 64
+
+typedef struct {
+  int8_t *codes;    /* device, [n_layers][n_pages][n_kv_heads][2][64][head_dim], 16-byte aligned */
+  float *scales;    /* device, [n_layers][n_pages][n_kv_heads][2], 8-byte aligned */
+  int n_layers, n_pages, n_kv_heads, head_dim;
+} gptoss_kv8_pool_t;
+
+/*
+ * Writes the key and value heads of T qkv rows into one layer of the cache (beside
+ * gptoss_kv_cache_write).  Per page, head and kind that gets rows: the scale becomes the smallest
+ * power of two s >= 2^-126 with max|x| <= 127 s over the new rows, or stays as it was if that is
+ * larger and the page already holds earlier tokens of the sequence; when it grows, the codes
+ * already there become rint(code * old / new) (ties to even).  A new code is rint(x / s).  Powers
+ * of two keep every step of this exact except the one rounding, and bound what repeated growth
+ * can cost: each regrowth at least doubles the scale, so all earlier roundings together stay below
+ * one step of the final scale.  A page whose slot 0 is written starts afresh, whatever it held.
+ * NaN is stored as 0, infinities as the largest finite fp32.  Rows whose position has no page are
+ * skipped; slots behind the last row are left as they were.
+ */
+GPTOSS_API int gptoss_kv8_append(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int layer, int T,
+                                 const void *qkv, gptoss_dtype_t qkv_dtype, long row_stride,
+                                 int n_q_heads, int n_seqs, const int *row_start, const int *kv_len,
+                                 const int *pages, int pages_stride, int max_new, unsigned flags);
+
+/*
+ * Attention of T qkv rows over one layer of the cache, which must already hold them
+ * (gptoss_kv8_append first): for query head h of a row at position p
+ *     z_t = scale * q_h . k_t      over the tokens t the row sees
+ *     out[row, h] = sum_t exp(z_t) v_t / (sum_t exp(z_t) + exp(sinks[h]))
+ * A row sees t <= p, and with window > 0 only t > p - window or t < n_first (the first tokens stay
+ * visible); tokens without a page are not seen by anybody.  sinks (fp32, one logit per query head,
+ * may be NULL) takes part in the denominator only (run.cpp:611-636 of the reference).  Where nothing
+ * is seen the output is 0; otherwise a query head with a NaN or an infinity in it gives NaN, and
+ * shows in no other output.  window 0 means no window.  Query head h reads key/value head
+ * h / (n_q_heads / n_kv_heads).  out has n_q_heads * head_dim values per row; rows that belong to no
+ * sequence are left as they were.
+ * Products are taken on the tensor cores with the codes as they are (exact in fp16); fp32 rows
+ * (qkv_dtype GPTOSS_F32) and the softmax weights that go with them are carried as two fp16 parts, so
+ * that the result has fp32's accuracy; sums are fp32.
+ * workspace: gptoss_kv8_attention_workspace bytes (for the same arguments on the same device),
+ * 16-byte aligned, contents irrelevant; calls that may overlap in time need one each.
+ */
+GPTOSS_API int gptoss_kv8_attention(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int layer,
+                                    int T, const void *qkv, gptoss_dtype_t qkv_dtype, long row_stride,
+                                    int n_q_heads, int n_seqs, const int *row_start, const int *kv_len,
+                                    const int *pages, int pages_stride, int max_new, float scale,
+                                    int window, int n_first, const float *sinks, void *out,
+                                    gptoss_dtype_t out_dtype, long out_row_stride, void *workspace,
+                                    size_t workspace_bytes, unsigned flags);
+/* Bytes of workspace for a call with these sizes on the current device; 0 for arguments the call
+ * itself would refuse. */
+GPTOSS_API size_t gptoss_kv8_attention_workspace(const gptoss_kv8_pool_t *pool, int T, int n_q_heads,
+                                                 int n_seqs, int max_new);
+
+/*
+ * Pages.  refs[page] (device, n_pages) counts the table entries that name the page; 0 means free.
+ * A page asked for is always the lowest-numbered free one, requests served in list order, so the
+ * tables after a call depend on the tables before it alone.  All lists are device arrays.  Entries
+ * outside the table ([0, n_seqs)) are ignored (served 0).  served (may be NULL): 1 per request that
+ * was carried out, else 0.  The workspace (gptoss_kv8_pages_workspace bytes, 16-byte aligned,
+ * contents irrelevant) is not shared between calls that may overlap.
+ */
+
+/*
+ * Lets go of pages of n listed sequences.  window 0: all of them; the sequence is empty afterwards
+ * (entries -1, kv_len 0).  window > 0: only pages that no later token will see through that window
+ * and that hold none of the first n_first tokens (entries -1; kv_len stays), for a table whose
+ * layers are all windowed.  A sequence listed twice is let go of once.
+ */
+GPTOSS_API int gptoss_kv8_release(gptoss_stream_t stream, int n, const int *seqs, int n_seqs,
+                                  int *kv_len, int *pages, int pages_stride, int n_pages, int *refs,
+                                  int window, int n_first, unsigned flags);
+/*
+ * Gives n listed sequences the pages for their tokens kv_len .. new_len - 1 that have none yet
+ * (kv_len itself is the caller's to advance).  All or nothing per request: request i is served if
+ * the free pages suffice for it and all (valid) requests listed before it.  Not served: a sequence that
+ * was listed before, new_len beyond the table's width.
+ */
+GPTOSS_API int gptoss_kv8_reserve(gptoss_stream_t stream, int n, const int *seqs, const int *new_len,
+                                  int n_seqs, const int *kv_len, int *pages, int pages_stride,
+                                  int n_pages, int *refs, int *served, void *workspace,
+                                  size_t workspace_bytes, unsigned flags);
+/*
+ * Makes children[i] a copy of parents[i]: its full pages are shared (refs + 1), a last page that is
+ * not full is copied, in every layer, into a free page of its own.  Pages a parent reserved ahead
+ * are not taken over.  Not served: a child that is not empty (kv_len 0, no pages), that was listed
+ * before or that is a parent in the same call, a parent whose kv_len is outside the table, or no free page left.  A parent may be
+ * listed any number of times.
+ */
+GPTOSS_API int gptoss_kv8_fork(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int n,
+                               const int *parents, const int *children, int n_seqs, int *kv_len,
+                               int *pages, int pages_stride, int *refs, int *served,
+                               void *workspace, size_t workspace_bytes, unsigned flags);
+/*
+ * Moves the live pages together: with n_live pages in use, the k-th lowest of those numbered n_live or
+ * more moves (in every layer) into the k-th lowest free page below n_live; tables and refs follow.
+ * remap[page] (n_pages): its new number, -1 for a page that was free.  n_live_out: one int.
+ */
+GPTOSS_API int gptoss_kv8_compact(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int n_seqs,
+                                  int *pages, int pages_stride, int *refs, int *remap, int *n_live_out,
+                                  void *workspace, size_t workspace_bytes, unsigned flags);
+/*
+ * Copies n pages (codes and scales, every layer): dst[i] receives src[i].  Pairs that name a page
+ * outside the pool are skipped.  A dst may not be named twice, nor be a src of another pair.
+ */
+GPTOSS_API int gptoss_kv8_copy_pages(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int n,
+                                     const int *src, const int *dst, unsigned flags);
+/* Bytes of workspace of the three calls above that take one. */
+GPTOSS_API size_t gptoss_kv8_pages_workspace(int n_pages, int n_seqs);
+
 #ifdef __cplusplus
 }
 #endif

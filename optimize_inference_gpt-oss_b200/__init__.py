@@ -55,6 +55,12 @@ class ChainConfig(C.Structure):
         return (self.n_q_heads + 2 * self.n_kv_heads) * self.head_dim
 
 
+class KV8Pool(C.Structure):
+    """gptoss_kv8_pool_t: the 8-bit paged cache's storage, device pointers owned by the caller."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("n_layers", C.c_int), ("n_pages", C.c_int),
+                ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
 _p, _i, _l, _z, _f, _u = C.c_void_p, C.c_int, C.c_long, C.c_size_t, C.c_float, C.c_uint
 
 # name -> (restype, argtypes); mirrors include/gptoss_kernels.h and include/gptoss_engine.h
@@ -83,6 +89,16 @@ PROTOTYPES = {
     "gptoss_argmax_keys_finish": (_i, [_p, _i, _p, _p, _u]),
     "gptoss_argmax_slices": (_i, [_i, _l, _i, _i]),
     "gptoss_argmax_noalloc": (_i, [_p, _i, _p, _i, _l, _l, _p]),
+    "gptoss_kv8_append": (_i, [_p, C.POINTER(KV8Pool), _i, _i, _p, _i, _l, _i, _i, _p, _p, _p, _i, _i, _u]),
+    "gptoss_kv8_attention": (_i, [_p, C.POINTER(KV8Pool), _i, _i, _p, _i, _l, _i, _i, _p, _p, _p, _i, _i, _f, _i, _i, _p,
+                                  _p, _i, _l, _p, _z, _u]),
+    "gptoss_kv8_attention_workspace": (_z, [C.POINTER(KV8Pool), _i, _i, _i, _i]),
+    "gptoss_kv8_release": (_i, [_p, _i, _p, _i, _p, _p, _i, _i, _p, _i, _i, _u]),
+    "gptoss_kv8_reserve": (_i, [_p, _i, _p, _p, _i, _p, _p, _i, _i, _p, _p, _p, _z, _u]),
+    "gptoss_kv8_fork": (_i, [_p, C.POINTER(KV8Pool), _i, _p, _p, _i, _p, _p, _i, _p, _p, _p, _z, _u]),
+    "gptoss_kv8_compact": (_i, [_p, C.POINTER(KV8Pool), _i, _p, _i, _p, _p, _p, _p, _z, _u]),
+    "gptoss_kv8_copy_pages": (_i, [_p, C.POINTER(KV8Pool), _i, _p, _p, _u]),
+    "gptoss_kv8_pages_workspace": (_z, [_i, _i]),
     "gptoss_device_count": (_i, [C.POINTER(_i)]),
     "gptoss_device_set": (_i, [_i]),
     "gptoss_device_name": (_i, [_i, C.c_char_p, _i]),
@@ -340,6 +356,73 @@ def argmax_noalloc(T, logits, dtype, V, row_stride, out, stream=None):
     """gptoss_argmax without caller scratch: the merge words sit in a fixed array inside the
     library, so at most ARGMAX_NOALLOC_MAX_ROWS rows per call and no overlapping calls per GPU."""
     check(load().gptoss_argmax_noalloc(stream, T, _ptr(logits), dtype, V, row_stride, _ptr(out)), "argmax_noalloc")
+
+
+# ---- the 8-bit paged cache --------------------------------------------------------
+
+KV8_PAGE = 64
+
+
+def kv8_pool(codes, scales, n_layers, n_pages, n_kv_heads, head_dim) -> KV8Pool:
+    return KV8Pool(_ptr(codes), _ptr(scales), n_layers, n_pages, n_kv_heads, head_dim)
+
+
+def kv8_append(pool, layer, T, qkv, dtype, row_stride, n_q, n_seqs, row_start, kv_len, pages, pages_stride, max_new,
+               flags=0, stream=None):
+    check(load().gptoss_kv8_append(stream, C.byref(pool), layer, T, _ptr(qkv), dtype, row_stride, n_q, n_seqs,
+                                   _ptr(row_start), _ptr(kv_len), _ptr(pages), pages_stride, max_new, flags), "kv8_append")
+
+
+def kv8_attention(pool, layer, T, qkv, dtype, row_stride, n_q, n_seqs, row_start, kv_len, pages, pages_stride, max_new,
+                  scale, window, n_first, sinks, out, out_dtype, out_stride, workspace, workspace_bytes, flags=0,
+                  stream=None):
+    check(load().gptoss_kv8_attention(stream, C.byref(pool), layer, T, _ptr(qkv), dtype, row_stride, n_q, n_seqs,
+                                      _ptr(row_start), _ptr(kv_len), _ptr(pages), pages_stride, max_new, scale, window,
+                                      n_first, _ptr(sinks), _ptr(out), out_dtype, out_stride, _ptr(workspace),
+                                      workspace_bytes, flags), "kv8_attention")
+
+
+def kv8_attention_workspace(pool, T, n_q, n_seqs, max_new) -> int:
+    return int(load().gptoss_kv8_attention_workspace(C.byref(pool), T, n_q, n_seqs, max_new))
+
+
+def kv8_release(n, seqs, n_seqs, kv_len, pages, pages_stride, n_pages, refs, window=0, n_first=0, flags=0, stream=None):
+    check(load().gptoss_kv8_release(stream, n, _ptr(seqs), n_seqs, _ptr(kv_len), _ptr(pages), pages_stride, n_pages,
+                                    _ptr(refs), window, n_first, flags), "kv8_release")
+
+
+def kv8_reserve(n, seqs, new_len, n_seqs, kv_len, pages, pages_stride, n_pages, refs, served, workspace, workspace_bytes,
+                flags=0, stream=None):
+    check(load().gptoss_kv8_reserve(stream, n, _ptr(seqs), _ptr(new_len), n_seqs, _ptr(kv_len), _ptr(pages), pages_stride,
+                                    n_pages, _ptr(refs), _ptr(served), _ptr(workspace), workspace_bytes, flags),
+          "kv8_reserve")
+
+
+def kv8_fork(pool, n, parents, children, n_seqs, kv_len, pages, pages_stride, n_pages, refs, served, workspace,
+             workspace_bytes, flags=0, stream=None):
+    if n_pages != pool.n_pages:
+        raise GptossError(ERR_BAD_ARG, "kv8_fork: the table's pages are not the pool's")
+    check(load().gptoss_kv8_fork(stream, C.byref(pool), n, _ptr(parents), _ptr(children), n_seqs, _ptr(kv_len),
+                                 _ptr(pages), pages_stride, _ptr(refs), _ptr(served), _ptr(workspace), workspace_bytes,
+                                 flags), "kv8_fork")
+
+
+def kv8_compact(pool, n_seqs, kv_len, pages, pages_stride, n_pages, refs, remap, n_live, workspace, workspace_bytes,
+                flags=0, stream=None):
+    """kv_len is not touched (a page's number is not part of a length); it is taken so that the
+    page calls share one argument list."""
+    if n_pages != pool.n_pages:
+        raise GptossError(ERR_BAD_ARG, "kv8_compact: the table's pages are not the pool's")
+    check(load().gptoss_kv8_compact(stream, C.byref(pool), n_seqs, _ptr(pages), pages_stride, _ptr(refs), _ptr(remap),
+                                    _ptr(n_live), _ptr(workspace), workspace_bytes, flags), "kv8_compact")
+
+
+def kv8_copy_pages(pool, n, src, dst, flags=0, stream=None):
+    check(load().gptoss_kv8_copy_pages(stream, C.byref(pool), n, _ptr(src), _ptr(dst), flags), "kv8_copy_pages")
+
+
+def kv8_pages_workspace(n_pages, n_seqs) -> int:
+    return int(load().gptoss_kv8_pages_workspace(n_pages, n_seqs))
 
 
 def build_rope_tables(n_pos, head_dim=64, theta=150000.0, factor=32.0, orig_ctx=4096.0,

@@ -1,0 +1,235 @@
+// Appending rows to the 8-bit paged cache (gptoss_kv8_append).
+//
+// For every page that gets rows, and for each key/value head and kind (key, value) of it:
+//     top = max |x| over the page's new rows          s' = the smallest 2^e >= 2^-126 with top <= 127 s'
+//     s   = s', or max(s', old scale) if the page holds earlier tokens
+//     earlier codes <- rint(code * old / s) where s grew;   new codes = rint(x / s)
+// Dividing by a power of two is exact, so the result is defined to the bit whatever the order of
+// the loads.
+//
+// One group of lanes owns one (page, head, kind), so nothing is shared between groups and there
+// are no atomics.  What bounds it: at prompt lengths the rows' bytes (2 of bf16 in, 1 of codes out
+// per element), which a block of 128 lanes holds in registers between the two passes (maximum,
+// then codes) so that they are read once; in a decode step, latency -- a warp per group, four
+// groups to a block, and a chain of four dependent loads (lengths, table entry, row, scale).
+#include "kv8.cuh"
+
+namespace gptoss {
+namespace kv8 {
+namespace {
+
+// |x| of a value to be stored: a NaN counts as 0, an infinity as the largest finite value.
+__device__ __forceinline__ float storable(float x) {
+  return x != x ? 0.0f : fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f);
+}
+
+// Exponent field (1 .. 249) of the smallest power of two s >= 2^-126 with top <= 127 s; 0 for top = 0.
+// top = 1.m * 2^(E - 127) and 127 = 1.984375 * 2^6 (mantissa field 0x7e0000).
+__device__ __forceinline__ int scale_field(float top) {
+  const uint32_t u = __float_as_uint(top);
+  if (u == 0)
+    return 0;
+  const int field = (int)(u >> 23) - 6 + ((u & 0x7fffffu) > 0x7e0000u);
+  return field < 1 ? 1 : field;
+}
+__device__ __forceinline__ float power_of_field(int field) { return __uint_as_float((uint32_t)field << 23); }
+
+template <typename QT> struct Eight; // eight stored values, as they lie in memory
+template <> struct Eight<float> {
+  uint4 a, b;
+  __device__ __forceinline__ Vec8 floats() const { return floats_of(a, b); }
+};
+template <> struct Eight<uint16_t> {
+  uint4 a;
+  __device__ __forceinline__ Vec8 floats() const { return widen8(a); }
+};
+template <bool VEC> __device__ __forceinline__ Eight<float> load_eight(const float *p) {
+  if constexpr (VEC)
+    return {ld_stream(p), ld_stream(p + 4)};
+  else {
+    const uint32_t *u = reinterpret_cast<const uint32_t *>(p);
+    return {make_uint4(u[0], u[1], u[2], u[3]), make_uint4(u[4], u[5], u[6], u[7])};
+  }
+}
+template <bool VEC> __device__ __forceinline__ Eight<uint16_t> load_eight(const uint16_t *p) {
+  if constexpr (VEC)
+    return {ld_stream(p)};
+  else
+    return {make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16,
+                       p[6] | (uint32_t)p[7] << 16)};
+}
+
+__device__ __forceinline__ uint32_t pack_codes(const float *v, float inverse) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    r |= ((uint32_t)__float2int_rn(v[i] * inverse) & 0xffu) << (8 * i);
+  return r;
+}
+__device__ __forceinline__ uint32_t rescale_codes(uint32_t w, float keep) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    r |= ((uint32_t)__float2int_rn((float)(int8_t)(w >> (8 * i)) * keep) & 0xffu) << (8 * i);
+  return r;
+}
+
+// GROUP lanes per (page, head, kind); a block of 128 threads holds 128 / GROUP of them.  blockIdx.x
+// counts (sequence, page) units, blockIdx.y groups of (head, kind).
+// Units: sequence s gets those from unit0(s) on, of which it needs (pages its rows touch) at most
+// rows / 64 + 2 (one where no sequence has more than one row).
+template <typename QT, int D, int GROUP, bool VEC>
+__global__ void __launch_bounds__(128)
+    append_rows(Layer cache, const QT *__restrict__ qkv, long row_stride, int n_q_heads, Rows rows) {
+  pdl_prologue();
+  constexpr int kLanesPerRow = D / 8, kRowsPerPass = GROUP / kLanesPerRow, kPasses = kPage / kRowsPerPass;
+  constexpr bool kHold = GROUP == 128; // a whole page of rows stays in the block's registers
+  const int lane = threadIdx.x % GROUP;
+  const int kind_head = blockIdx.y * (128 / GROUP) + threadIdx.x / GROUP;
+  const bool active = kind_head < 2 * cache.n_kv_heads;
+  const int kind = kind_head & 1, head = kind_head >> 1;
+
+  const int unit = blockIdx.x, one = rows.max_new == 1;
+  auto unit0 = [&](int s) { return one ? s : rows.start(s) / kPage + 2 * s; };
+  const int s = one ? unit : rows.find(unit, unit0);
+  const Rows::Span sp = rows.span(s);
+  const int begin = max(sp.pos, 0), end = sp.pos + sp.q; // positions to be written
+  const int p = begin / kPage + unit - unit0(s);         // table column
+  if (unit < unit0(s) || begin >= end || p >= rows.pages_stride || p * kPage >= end)
+    return;
+  const int page = cache.checked(__ldg(rows.pages + (size_t)s * rows.pages_stride + p));
+  if (page < 0)
+    return;
+  const int slot0 = max(begin - p * kPage, 0), slot1 = min(end - p * kPage, kPage); // slots [slot0, slot1) get rows
+  const int element = (lane % kLanesPerRow) * 8, sub = lane / kLanesPerRow;
+  const QT *src = qkv + (size_t)(sp.row + (p * kPage - sp.pos)) * row_stride; // the row of slot 0
+  src += (size_t)(n_q_heads + kind * cache.n_kv_heads + (active ? head : 0)) * D + element;
+
+  Eight<QT> held[kHold ? kPasses : 1];
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPasses; i++) {
+    const int slot = (kHold ? 0 : slot0) + i * kRowsPerPass + sub;
+    if (kHold ? (slot >= slot0 && slot < slot1) : slot < slot1) {
+      const Eight<QT> e = load_eight<VEC>(src + (long)slot * row_stride);
+      if constexpr (kHold)
+        held[i] = e;
+      const Vec8 v = e.floats();
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        top = fmaxf(top, fabsf(storable(v.v[j])));
+    }
+    if (!kHold && slot0 + (i + 1) * kRowsPerPass >= slot1)
+      break;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if constexpr (GROUP == 128) {
+    __shared__ float part[4];
+    if ((threadIdx.x & 31) == 0)
+      part[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  }
+  if (!active)
+    return;
+
+  float *scale_at = cache.scale(page, head) + kind;
+  int8_t *block = cache.block<D>(page, head) + kind * kPage * D + element;
+  const int field = scale_field(top);
+  float scale = power_of_field(field), inverse = field ? power_of_field(254 - field) : 0.0f;
+  if (slot0 > 0) { // the page holds earlier tokens: its scale never shrinks
+    const float old = *scale_at;
+    if (old >= scale) {
+      scale = old;
+      inverse = old > 0.0f ? 1.0f / old : 0.0f;
+    } else if (old > 0.0f) {
+      const float keep = old * inverse;
+      for (int slot = sub; slot < slot0; slot += kRowsPerPass) {
+        uint2 *at = reinterpret_cast<uint2 *>(block + slot * D);
+        const uint2 w = *at;
+        *at = make_uint2(rescale_codes(w.x, keep), rescale_codes(w.y, keep));
+      }
+    }
+  }
+  if constexpr (GROUP == 128)
+    __syncthreads(); // every lane has read the old scale
+  else
+    __syncwarp();
+  if (lane == 0)
+    *scale_at = scale;
+#pragma unroll
+  for (int i = 0; i < kPasses; i++) {
+    const int slot = (kHold ? 0 : slot0) + i * kRowsPerPass + sub;
+    if (kHold ? (slot >= slot0 && slot < slot1) : slot < slot1) {
+      Vec8 v = kHold ? held[kHold ? i : 0].floats() : load_eight<VEC>(src + (long)slot * row_stride).floats();
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        v.v[j] = storable(v.v[j]);
+      *reinterpret_cast<uint2 *>(block + slot * D) = make_uint2(pack_codes(v.v, inverse), pack_codes(v.v + 4, inverse));
+    }
+    if (!kHold && slot0 + (i + 1) * kRowsPerPass >= slot1)
+      break;
+  }
+}
+
+template <typename QT, int D, bool VEC>
+void launch_append(cudaStream_t stream, Layer cache, const void *qkv, long row_stride, int n_q_heads, const Rows &rows) {
+  const int groups = 2 * cache.n_kv_heads;
+  const int units = rows.max_new == 1 ? rows.n_seqs : rows.T / kPage + 2 * rows.n_seqs;
+  const QT *q = static_cast<const QT *>(qkv);
+  // A warp per group while a pass of it (4 rows at 64 elements) or two cover a sequence's rows; above
+  // that the block that reads its rows once.
+  if (rows.max_new <= 8)
+    launch_kernel(append_rows<QT, D, 32, VEC>, dim3(units, (groups + 3) / 4), dim3(128), 0, stream, cache, q, row_stride,
+                  n_q_heads, rows);
+  else
+    launch_kernel(append_rows<QT, D, 128, VEC>, dim3(units, groups), dim3(128), 0, stream, cache, q, row_stride, n_q_heads,
+                  rows);
+}
+
+} // namespace
+} // namespace kv8
+} // namespace gptoss
+
+extern "C" int gptoss_kv8_append(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int layer, int T, const void *qkv,
+                                 gptoss_dtype_t qkv_dtype, long row_stride, int n_q_heads, int n_seqs,
+                                 const int *row_start, const int *kv_len, const int *pages, int pages_stride, int max_new,
+                                 unsigned flags) {
+  using namespace gptoss;
+  const PdlScope pdl(flags);
+  if (T < 0)
+    return GPTOSS_ERR_BAD_ARG;
+  if (const int st = kv8::check_pool(pool))
+    return st;
+  if (T == 0)
+    return GPTOSS_OK;
+  if (const int st = kv8::check_rows(pool, layer, T, qkv, qkv_dtype, row_stride, n_q_heads, n_seqs, row_start, kv_len,
+                                     pages, pages_stride, max_new))
+    return st;
+  if (2 * (long)pool->n_kv_heads > 65535)
+    return GPTOSS_ERR_UNSUPPORTED;
+  const int D = pool->head_dim;
+  GPTOSS_SPAN(qkv, strided_bytes(T, row_stride, (long)(n_q_heads + 2l * pool->n_kv_heads) * D, dtype_size(qkv_dtype)));
+  GPTOSS_SPAN(pool->codes, kv8::layer_codes(pool) * pool->n_layers);
+  GPTOSS_SPAN(pool->scales, kv8::layer_scales(pool) * pool->n_layers * 4);
+  GPTOSS_SPAN(row_start, ((size_t)n_seqs + 1) * 4);
+  GPTOSS_SPAN(kv_len, (size_t)n_seqs * 4);
+  GPTOSS_SPAN(pages, (size_t)n_seqs * pages_stride * 4);
+  const kv8::Layer cache = kv8::layer_of(pool, layer);
+  const kv8::Rows rows = {row_start, kv_len, pages, T, n_seqs, pages_stride, max_new > T ? T : max_new};
+  const bool vec = aligned16(qkv) && row_stride * (long)dtype_size(qkv_dtype) % 16 == 0;
+  if (!vec)
+    note_generic_launch();
+  const cudaStream_t s = as_stream(stream);
+#define GPTOSS_APPEND(QT, DD)                                                                                          \
+  (vec ? kv8::launch_append<QT, DD, true>(s, cache, qkv, row_stride, n_q_heads, rows)                                  \
+       : kv8::launch_append<QT, DD, false>(s, cache, qkv, row_stride, n_q_heads, rows))
+  if (qkv_dtype == GPTOSS_F32)
+    D == 64 ? GPTOSS_APPEND(float, 64) : GPTOSS_APPEND(float, 128);
+  else
+    D == 64 ? GPTOSS_APPEND(uint16_t, 64) : GPTOSS_APPEND(uint16_t, 128);
+#undef GPTOSS_APPEND
+  return launch_status();
+}
