@@ -81,10 +81,9 @@ __device__ __forceinline__ void value_factor(int e, uint32_t &mul, uint32_t &add
   mul = m * 0x10001u, add = a * 0x10001u;
 }
 
-// Row n of an 8-token tile of scores is token n with its lowest bit flipped in every other pair: the
-// four tokens that a lane multiplies values of then lie in different halves of a 128-byte line from
-// its neighbours'.
-__device__ __forceinline__ int token_of(int n) { return n ^ ((n >> 1) & 1); }
+// Row n of an 8-token tile of scores holds this token of the tile: the tokens whose values the lanes
+// of a quad load together are then neighbours (256 consecutive bytes per load).
+__device__ __forceinline__ int token_of(int n) { return (n >> 1) + 4 * (n & 1); }
 
 template <typename QT> __device__ __forceinline__ void load4(const QT *p, bool vec, float (&v)[4]) {
   if (vec) {
@@ -118,233 +117,223 @@ template <typename QT> __device__ __forceinline__ void store4(const Call<QT> &a,
   }
 }
 
-// A row's sum and maximum joined with its head's sink logit; what the row's values are to be divided by.
-__device__ __forceinline__ void join_sink(const float *sinks, int h, float &m, float &l) {
-  if (!sinks || l == 0.0f)
-    return;
-  const float z = fminf(__ldg(sinks + h) * kLog2e, 3e38f), top = fmaxf(m, z);
-  l = l * fast_exp2(m - top) + fast_exp2(z - top);
-  m = top;
-}
-
-template <typename QT, int D, int MT> struct TokenKernel {
-  static constexpr bool kSplit = sizeof(QT) == 4;            // two fp16 parts
-  static constexpr int CH = (D == 64 ? 64 : 32) / MT;        // tokens of a step
-  static constexpr int kSteps = kPage / CH;                  // steps of a page
-  static constexpr int NT = CH / 8, KK = CH / 16, KS = D / 16, DV = D / 8;
-  static constexpr int kRows = 16 * MT;
-  static constexpr int kPitch = D + 4;                       // floats of a row in shared memory
+// Scores and outputs are kept transposed (tokens x rows, elements x rows): the 8-wide side of the
+// matrix instruction is the rows', so that 8 rows (a group of 8 query heads and one token) waste nothing.
+template <typename QT, int D, int RB> struct TokenKernel {
+  static constexpr bool kSplit = sizeof(QT) == 4;                     // two fp16 parts
+  static constexpr int CH = (D == 64 ? 64 : 32) / (RB == 4 ? 2 : 1);  // tokens of a step
+  static constexpr int kSteps = kPage / CH;                           // steps of a page
+  static constexpr int TT = CH / 16, KS = D / 16, DT = D / 16;        // 16-token tiles, products of a score, 16-element tiles
+  static constexpr int kRows = 8 * RB;
+  static constexpr int kPitch = D + 4; // floats of a row in shared memory
   static constexpr int kSmem = kTokenWarps * kRows * (kPitch * 4 + 8);
   using VWord = typename std::conditional<D == 64, uint2, uint4>::type;
 
-  uint4 K[NT][D / 64];
-  VWord V[KK][4];
-  uint32_t q[MT][KS][4], q_rest[kSplit ? MT : 1][kSplit ? KS : 1][4];
-  float row_factor[MT][2], m[MT][2], l[MT][2], o[MT][DV][4];
-  int row_pos[MT][2]; // -1: no such row
-  bool bad[MT][2];
+  uint4 K[TT][2][D / 64]; // [tile][token g / g + 8]
+  VWord V[TT][4];         // [tile][the four tokens of a lane]
+  uint32_t q[RB][KS][2], q_rest[kSplit ? RB : 1][kSplit ? KS : 1][2];
+  float row_factor[RB][2], m[RB][2], l[RB][2], o[RB][DT][4]; // of rows 2t, 2t + 1 of each 8
+  int row_pos[RB][2];                                        // -1: no such row
   int value_exp;
 
   __device__ __forceinline__ void load_keys(const int8_t *block, int step) {
     const int lane = threadIdx.x & 31, n = token_of(lane >> 2), t = lane & 3;
 #pragma unroll
-    for (int i = 0; i < NT; i++)
+    for (int i = 0; i < TT; i++)
 #pragma unroll
-      for (int j = 0; j < D / 64; j++)
-        K[i][j] = ld_stream(block + (size_t)(step * CH + 8 * i + n) * D + j * 64 + t * 16);
+      for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int j = 0; j < D / 64; j++)
+          K[i][half][j] = ld_stream(block + (size_t)(step * CH + 16 * i + 8 * half + n) * D + j * 64 + t * 16);
   }
   __device__ __forceinline__ void load_values(const int8_t *block, int step) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int kk = 0; kk < KK; kk++)
+    for (int i = 0; i < TT; i++)
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const int token = step * CH + 16 * kk + 8 * (c >> 1) + token_of(2 * t + (c & 1));
+      for (int c = 0; c < 4; c++) { // rows 2t, 2t + 1, 2t + 8, 2t + 9 of the tile
+        const int token = step * CH + 16 * i + 8 * (c >> 1) + token_of(2 * t + (c & 1));
         const int8_t *p = block + (size_t)(kPage + token) * D + g * (D / 8);
         if constexpr (D == 64)
-          asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(V[kk][c].x), "=r"(V[kk][c].y) : "l"(p));
+          asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(V[i][c].x), "=r"(V[i][c].y) : "l"(p));
         else
-          V[kk][c] = ld_stream(p);
+          V[i][c] = ld_stream(p);
       }
   }
 
-  // The group's queries as left operands; a row's elements in the order that K's lanes have them.
+  // The group's queries as right operands (lane: row g), a row's elements in the order that K's lanes
+  // have them; then what a lane keeps of the rows it has scores of (2t, 2t + 1).
   __device__ __forceinline__ void load_queries(const Call<QT> &a, const Rows::Span &sp, int head, int row0) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, R = sp.q * a.group;
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int b = 0; b < RB; b++) {
+      const int r = row0 + 8 * b + g;
+      const bool is = r < R;
+      const int token = is ? r / a.group : 0, h = head * a.group + (is ? r % a.group : 0);
+      const QT *p = a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D + 16 * t;
+      float v[KS][4], top = 0.0f;
+      bool odd = false;
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int r = row0 + 16 * mt + 8 * half + g;
-        const bool is = r < R;
-        const int token = is ? r / a.group : 0, h = head * a.group + (is ? r % a.group : 0);
-        row_pos[mt][half] = is ? sp.pos + token : -1;
-        const QT *p = a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D + 16 * t;
-        float v[KS][4], top = 0.0f;
-        bool odd = false;
+      for (int j = 0; j < KS; j++)
+        load4(p + (j / 4) * 64 + (j % 4) * 4, a.q_vec, v[j]);
 #pragma unroll
-        for (int j = 0; j < KS; j++) {
-          load4(p + (j / 4) * 64 + (j % 4) * 4, a.q_vec, v[j]);
+      for (int j = 0; j < KS; j++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            v[j][e] = is ? v[j][e] : 0.0f;
-            odd = odd || !(fabsf(v[j][e]) <= 3.402823466e38f);
-            top = fmaxf(top, fabsf(v[j][e]));
-          }
+        for (int e = 0; e < 4; e++) {
+          odd = odd || !(fabsf(v[j][e]) <= 3.402823466e38f);
+          top = fmaxf(top, fabsf(v[j][e]));
         }
 #pragma unroll
-        for (int s = 1; s < 4; s <<= 1) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-          odd = __shfl_xor_sync(0xffffffffu, (int)odd, s) || odd;
-        }
-        bad[mt][half] = odd;
-        // largest |q| into [2^13, 2^14); rows too small for the exponent keep a factor of 2^126
-        const int up = odd || top == 0.0f ? 0 : min(13 - (exponent_field(top) - 127), 126);
-        const float f = two_to(max(up, -126)) * (a.scale < 0.0f ? -1.0f : 1.0f);
-        row_factor[mt][half] = fabsf(a.scale) * kLog2e * two_to(-max(up, -126));
-#pragma unroll
-        for (int j = 0; j < KS; j++)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            const float x = odd ? 0.0f : v[j][e] * f, y = odd ? 0.0f : v[j][e + 1] * f;
-            const uint32_t w = pack_f16(x, y);
-            q[mt][j][e + half] = w; // a0/a1: elements 0,1; a2/a3: elements 2,3
-            if constexpr (kSplit)
-              q_rest[mt][j][e + half] = pack_rest(w, x, y);
-          }
+      for (int x = 1; x < 4; x <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        odd = __shfl_xor_sync(0xffffffffu, (int)odd, x) || odd;
       }
+      // largest |q| into [2^13, 2^14); rows too small for the exponent keep a factor of 2^126
+      const int up = odd || top == 0.0f ? 0 : max(min(13 - (exponent_field(top) - 127), 126), -126);
+      const float f = odd || !is ? 0.0f : two_to(up) * (a.scale < 0.0f ? -1.0f : 1.0f);
+#pragma unroll
+      for (int j = 0; j < KS; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const float x = odd || !is ? 0.0f : v[j][2 * e] * f, y = odd || !is ? 0.0f : v[j][2 * e + 1] * f;
+          q[b][j][e] = pack_f16(x, y);
+          if constexpr (kSplit)
+            q_rest[b][j][e] = pack_rest(q[b][j][e], x, y);
+        }
+      const float factor = odd ? NAN : fabsf(a.scale) * kLog2e * two_to(-up);
+      const int pos = is ? sp.pos + token : -1;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        row_factor[b][e] = __shfl_sync(0xffffffffu, factor, (2 * t + e) * 4);
+        row_pos[b][e] = __shfl_sync(0xffffffffu, pos, (2 * t + e) * 4);
+      }
+    }
   }
 
   __device__ __forceinline__ void begin() {
     value_exp = 0;
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int b = 0; b < RB; b++)
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        m[mt][half] = -INFINITY, l[mt][half] = 0.0f;
+      for (int e = 0; e < 2; e++) {
+        m[b][e] = -INFINITY, l[b][e] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < DV; j++)
-          o[mt][j][2 * half] = o[mt][j][2 * half + 1] = 0.0f;
+        for (int j = 0; j < DT; j++)
+          o[b][j][e] = o[b][j][2 + e] = 0.0f;
       }
   }
 
-  __device__ __forceinline__ void scores(float (&s)[MT][NT][4]) {
+  __device__ __forceinline__ void scores(float (&s)[RB][TT][4]) {
 #pragma unroll
-    for (int i = 0; i < NT; i++) {
+    for (int i = 0; i < TT; i++) {
 #pragma unroll
-      for (int mt = 0; mt < MT; mt++)
-        s[mt][i][0] = s[mt][i][1] = s[mt][i][2] = s[mt][i][3] = 0.0f;
+      for (int b = 0; b < RB; b++)
+        s[b][i][0] = s[b][i][1] = s[b][i][2] = s[b][i][3] = 0.0f;
 #pragma unroll
       for (int j = 0; j < KS; j++) {
-        const uint4 w4 = K[i][j / 4];
-        const uint32_t u = biased(j % 4 == 0 ? w4.x : j % 4 == 1 ? w4.y : j % 4 == 2 ? w4.z : w4.w);
-        const uint32_t b0 = minus_1152(low_pair(u)), b1 = minus_1152(high_pair(u));
+        const uint32_t u = biased(word(K[i][0][j / 4], j % 4)), v = biased(word(K[i][1][j / 4], j % 4));
+        const uint32_t k[4] = {minus_1152(low_pair(u)), minus_1152(low_pair(v)), minus_1152(high_pair(u)),
+                               minus_1152(high_pair(v))};
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-          mma_f16(s[mt][i], q[mt][j], b0, b1);
+        for (int b = 0; b < RB; b++) {
+          mma_f16(s[b][i], k, q[b][j][0], q[b][j][1]);
           if constexpr (kSplit)
-            mma_f16(s[mt][i], q_rest[mt][j], b0, b1);
+            mma_f16(s[b][i], k, q_rest[b][j][0], q_rest[b][j][1]);
         }
       }
     }
   }
 
   // s becomes the weights of the step's tokens first_token ..
-  __device__ __forceinline__ void weigh(float (&s)[MT][NT][4], float key_scale, int v_exp, bool masked, int first_token,
-                                        int window, int n_first) {
-    const int t = threadIdx.x & 3;
+  template <bool MASKED>
+  __device__ __forceinline__ void weigh(float (&s)[RB][TT][4], float key_scale, int v_exp, int first_token, int window,
+                                        int n_first) {
+    const int first = first_token + token_of((threadIdx.x & 31) >> 2); // tile i's rows g, g + 8: tokens first + 16 i, + 8
     bool moved = v_exp > value_exp;
-    float fade[MT][2];
+    float fade[RB][2];
     const float beta = moved ? two_to(value_exp - v_exp) : 1.0f;
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int b = 0; b < RB; b++)
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        uint32_t seen = 0xffffffffu;
+      for (int e = 0; e < 2; e++) {
+        uint32_t seen = 0;
         float top = -INFINITY;
-        if (masked) {
-          seen = 0;
-          const int pos = row_pos[mt][half];
 #pragma unroll
-          for (int i = 0; i < NT; i++)
+        for (int i = 0; i < TT; i++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-              const int token = first_token + 8 * i + token_of(2 * t + e);
+          for (int half = 0; half < 2; half++) {
+            if constexpr (MASKED) {
+              const int token = first + 16 * i + 8 * half, pos = row_pos[b][e];
               const bool ok = token <= pos && (window <= 0 || token > pos - window || token < n_first);
-              seen |= (uint32_t)ok << (2 * i + e);
-              top = fmaxf(top, ok ? s[mt][i][2 * half + e] : -INFINITY);
+              seen |= (uint32_t)ok << (2 * i + half);
+              top = fmaxf(top, ok ? s[b][i][2 * half + e] : -INFINITY);
+            } else {
+              top = fmaxf(top, s[b][i][2 * half + e]);
             }
-        } else {
+          }
 #pragma unroll
-          for (int i = 0; i < NT; i++)
-            top = fmaxf(top, fmaxf(s[mt][i][2 * half], s[mt][i][2 * half + 1]));
-        }
-#pragma unroll
-        for (int x = 1; x < 4; x <<= 1)
+        for (int x = 4; x < 32; x <<= 1)
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float f = row_factor[mt][half] * key_scale;
-        const float now = top > -INFINITY ? fmaxf(m[mt][half], top * f) : m[mt][half];
+        const float f = row_factor[b][e] * key_scale;
+        const float now = top > -INFINITY ? fmaxf(m[b][e], top * f) : m[b][e];
         const float base = now > -INFINITY ? now : 0.0f;
-        const float a = fast_exp2(m[mt][half] - base), off = (float)kWeightBits - base;
-        m[mt][half] = now;
+        const float a = fast_exp2(m[b][e] - base), off = (float)kWeightBits - base;
+        m[b][e] = now;
         moved = moved || a != 1.0f;
-        fade[mt][half] = a * beta;
+        fade[b][e] = a * beta;
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NT; i++)
+        for (int i = 0; i < TT; i++)
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float p = fast_exp2(fmaf(s[mt][i][2 * half + e], f, off));
-            if (masked)
-              p = seen >> (2 * i + e) & 1 ? p : 0.0f;
-            s[mt][i][2 * half + e] = p;
+          for (int half = 0; half < 2; half++) {
+            float p = fast_exp2(fmaf(s[b][i][2 * half + e], f, off));
+            if constexpr (MASKED)
+              p = seen >> (2 * i + half) & 1 ? p : 0.0f;
+            s[b][i][2 * half + e] = p;
             sum += p;
           }
-        l[mt][half] = l[mt][half] * a + sum;
+        l[b][e] = fmaf(l[b][e], a, sum);
       }
     value_exp = max(value_exp, v_exp);
     if (__any_sync(0xffffffffu, moved))
 #pragma unroll
-      for (int mt = 0; mt < MT; mt++)
+      for (int b = 0; b < RB; b++)
 #pragma unroll
-        for (int j = 0; j < DV; j++)
-          o[mt][j][0] *= fade[mt][0], o[mt][j][1] *= fade[mt][0], o[mt][j][2] *= fade[mt][1], o[mt][j][3] *= fade[mt][1];
+        for (int j = 0; j < DT; j++)
+          o[b][j][0] *= fade[b][0], o[b][j][1] *= fade[b][1], o[b][j][2] *= fade[b][0], o[b][j][3] *= fade[b][1];
   }
 
-  __device__ __forceinline__ void add_values(const float (&s)[MT][NT][4], int v_exp) {
+  __device__ __forceinline__ void add_values(const float (&s)[RB][TT][4], int v_exp) {
     uint32_t mul, add;
     value_factor(v_exp == 0 ? -99 : v_exp - value_exp + kValueBits, mul, add);
 #pragma unroll
-    for (int kk = 0; kk < KK; kk++) {
-      uint32_t p[MT][4], rest[kSplit ? MT : 1][4];
+    for (int i = 0; i < TT; i++) {
+      uint32_t p[RB][2], rest[kSplit ? RB : 1][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; mt++)
+      for (int b = 0; b < RB; b++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) { // a0, a1: rows g, g + 8 of the first tile; a2, a3: of the second
-          const float x = s[mt][2 * kk + (r >> 1)][2 * (r & 1)], y = s[mt][2 * kk + (r >> 1)][2 * (r & 1) + 1];
-          p[mt][r] = pack_f16(x, y);
+        for (int half = 0; half < 2; half++) {
+          const uint32_t w = pack_f16(s[b][i][2 * half], s[b][i][2 * half + 1]);
+          p[b][half] = transposed(w);
           if constexpr (kSplit)
-            rest[mt][r] = pack_rest(p[mt][r], x, y);
+            rest[b][half] = transposed(pack_rest(w, s[b][i][2 * half], s[b][i][2 * half + 1]));
         }
 #pragma unroll
-      for (int w = 0; w < D / 32; w++) { // words of 4 elements
+      for (int w = 0; w < D / 32; w++) { // words of 4 elements: two 16-element tiles' rows g and g + 8
         uint32_t c[4];
 #pragma unroll
         for (int x = 0; x < 4; x++)
-          c[x] = biased(word(V[kk][x], w));
+          c[x] = biased(word(V[i][x], w));
 #pragma unroll
         for (int hi = 0; hi < 2; hi++) {
-          const uint32_t a = __byte_perm(c[0], c[1], hi ? 0x7362 : 0x5140), b = __byte_perm(c[2], c[3], hi ? 0x7362 : 0x5140);
+          const uint32_t x = __byte_perm(c[0], c[1], hi ? 0x7362 : 0x5140), y = __byte_perm(c[2], c[3], hi ? 0x7362 : 0x5140);
+          const uint32_t v[4] = {scaled_pair(low_pair(x), mul, add), scaled_pair(high_pair(x), mul, add),
+                                 scaled_pair(low_pair(y), mul, add), scaled_pair(high_pair(y), mul, add)};
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const uint32_t b0 = scaled_pair(e ? high_pair(a) : low_pair(a), mul, add);
-            const uint32_t b1 = scaled_pair(e ? high_pair(b) : low_pair(b), mul, add);
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-              mma_f16(o[mt][4 * w + 2 * hi + e], p[mt], b0, b1);
-              if constexpr (kSplit)
-                mma_f16(o[mt][4 * w + 2 * hi + e], rest[mt], b0, b1);
-            }
+          for (int b = 0; b < RB; b++) {
+            mma_f16(o[b][2 * w + hi], v, p[b][0], p[b][1]);
+            if constexpr (kSplit)
+              mma_f16(o[b][2 * w + hi], v, rest[b][0], rest[b][1]);
           }
         }
       }
@@ -354,8 +343,8 @@ template <typename QT, int D, int MT> struct TokenKernel {
   static __device__ __forceinline__ uint32_t word(uint4 v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
 
   // The columns [i0, i1) of an item, steps dealt to the block's warps in turn.
-  __device__ __forceinline__ void run(const Call<QT> &a, int s, int head, const Columns &cols, int i0, int i1, int min_pos,
-                                      int max_pos) {
+  __device__ __forceinline__ void run(const Call<QT> &a, const Rows::Span &sp, int s, int head, int row0, const Columns &cols,
+                                      int i0, int i1, int min_pos, int max_pos) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int end = i1 * kSteps;
     const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
@@ -368,16 +357,17 @@ template <typename QT, int D, int MT> struct TokenKernel {
         scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
     };
     begin();
-    int j = held;
-    if (j >= end)
-      return;
-    fetch();
-    int page = __shfl_sync(0xffffffffu, page_of, 0), at = 0;
-    float ks = __shfl_sync(0xffffffffu, scale_of.x, 0), vs = __shfl_sync(0xffffffffu, scale_of.y, 0);
-    if (page >= 0) {
-      load_keys(a.cache.template block<D>(page, head), j % kSteps);
-      load_values(a.cache.template block<D>(page, head), j % kSteps);
+    int j = held, at = 0, page = -1;
+    if (j < end) {
+      fetch();
+      page = __shfl_sync(0xffffffffu, page_of, 0);
+      if (page >= 0) {
+        load_keys(a.cache.template block<D>(page, head), j % kSteps);
+        load_values(a.cache.template block<D>(page, head), j % kSteps);
+      }
     }
+    load_queries(a, sp, head, row0); // while the first step's loads are on their way
+    float ks = __shfl_sync(0xffffffffu, scale_of.x, 0), vs = __shfl_sync(0xffffffffu, scale_of.y, 0);
     for (; j < end; j += kTokenWarps) {
       if (++at == 32) {
         held += 32 * kTokenWarps, at = 0;
@@ -386,15 +376,17 @@ template <typename QT, int D, int MT> struct TokenKernel {
       const int next = __shfl_sync(0xffffffffu, page_of, at), next_step = (j + kTokenWarps) % kSteps;
       const float next_ks = __shfl_sync(0xffffffffu, scale_of.x, at), next_vs = __shfl_sync(0xffffffffu, scale_of.y, at);
       const int8_t *next_block = a.cache.template block<D>(max(next, 0), head);
-      float w[MT][NT][4];
+      float w[RB][TT][4];
       if (page >= 0)
         scores(w);
       if (next >= 0)
         load_keys(next_block, next_step);
       if (page >= 0) {
         const int token = cols.at(j / kSteps) * kPage + (j % kSteps) * CH, v_exp = exponent_field(vs);
-        const bool all = token + CH - 1 <= min_pos && (a.window <= 0 || token > max_pos - a.window || token + CH <= a.n_first);
-        weigh(w, ks, v_exp, !all, token, a.window, a.n_first);
+        if (token + CH - 1 <= min_pos && (a.window <= 0 || token > max_pos - a.window || token + CH <= a.n_first))
+          weigh<false>(w, ks, v_exp, token, a.window, a.n_first);
+        else
+          weigh<true>(w, ks, v_exp, token, a.window, a.n_first);
         add_values(w, v_exp);
       }
       if (next >= 0)
@@ -412,57 +404,47 @@ template <typename QT, int D, int MT> struct TokenKernel {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const float unit = two_to(value_exp - 127 - kValueBits);
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int b = 0; b < RB; b++)
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        float sum = l[mt][half];
+      for (int e = 0; e < 2; e++) {
+        float sum = l[b][e];
 #pragma unroll
-        for (int x = 1; x < 4; x <<= 1)
+        for (int x = 4; x < 32; x <<= 1)
           sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        const int r = 16 * mt + 8 * half + g;
-        if (t == 0)
-          sml[warp * kRows + r] = make_float2(m[mt][half], bad[mt][half] && sum > 0.0f ? NAN : sum * two_to(-kWeightBits));
-        const float inverse = sum > 0.0f ? 1.0f / sum : 0.0f;
-        float *row = so + (warp * kRows + r) * kPitch;
+        const int r = 8 * b + 2 * t + e;
+        if (g == 0)
+          sml[warp * kRows + r] = make_float2(m[b][e], sum * two_to(-kWeightBits));
+        const float f = sum > 0.0f ? unit / sum : 0.0f;
+        float *row = so + (warp * kRows + r) * kPitch + g * (D / 8);
 #pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-          for (int j = 0; j < DV; j += 4)
-            *reinterpret_cast<float4 *>(row + (2 * t + n) * DV + j) =
-                make_float4(o[mt][j][2 * half + n] * inverse * unit, o[mt][j + 1][2 * half + n] * inverse * unit,
-                            o[mt][j + 2][2 * half + n] * inverse * unit, o[mt][j + 3][2 * half + n] * inverse * unit);
+        for (int j = 0; j < DT; j += 2)
+          *reinterpret_cast<float4 *>(row + 2 * j) =
+              make_float4(o[b][j][e] * f, o[b][j][2 + e] * f, o[b][j + 1][e] * f, o[b][j + 1][2 + e] * f);
       }
     __syncthreads();
     const int R = min(sp.q * a.group - row0, kRows);
     for (int i = threadIdx.x; i < R * (D / 4); i += kTokenWarps * 32) {
-      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-      float top = -INFINITY, sum = 0.0f;
+      const int r = i / (D / 4), d = (i % (D / 4)) * 4, h = head * a.group + (row0 + r) % a.group;
+      const bool sink = !piece_o && a.sinks;
+      const float z = sink ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY;
+      float2 ml[kTokenWarps];
+      float top = z, sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kTokenWarps; w++)
-        top = fmaxf(top, sml[w * kRows + r].x);
+      for (int w = 0; w < kTokenWarps; w++) {
+        ml[w] = sml[w * kRows + r];
+        top = fmaxf(top, ml[w].x);
+      }
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kTokenWarps; w++) {
-        const float2 ml = sml[w * kRows + r];
-        if (ml.y == 0.0f)
-          continue;
-        const float part = ml.y * fast_exp2(ml.x - top);
+        const float part = ml[w].y != 0.0f ? ml[w].y * fast_exp2(ml[w].x - top) : 0.0f; // a NaN passes
         const float4 x = *reinterpret_cast<const float4 *>(so + (w * kRows + r) * kPitch + d);
         sum += part;
         acc.x += part * x.x, acc.y += part * x.y, acc.z += part * x.z, acc.w += part * x.w;
       }
-      const int h = head * a.group + (row0 + r) % a.group;
-      if (!piece_o)
-        join_sink(a.sinks, h, top, sum);
-      // the weights above are relative to the warps' maximum, the sum now perhaps to the sink's
-      float f = sum != 0.0f ? 1.0f / sum : 0.0f;
-      if (!piece_o && a.sinks && sum != 0.0f) {
-        float before = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kTokenWarps; w++)
-          before = fmaxf(before, sml[w * kRows + r].x);
-        f *= fast_exp2(before - top);
-      }
+      if (sink && sum != 0.0f)
+        sum += fast_exp2(z - top);
+      const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
       acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
       if (piece_o) {
         *reinterpret_cast<float4 *>(piece_o + (size_t)r * D + d) = acc;
@@ -478,8 +460,7 @@ template <typename QT, int D, int MT> struct TokenKernel {
 
   __device__ __forceinline__ void item(const Call<QT> &a, const Rows::Span &sp, int s, int head, int rg, const Columns &cols,
                                        int i0, int i1, int min_pos, int max_pos, float *piece_o, float2 *piece_ml) {
-    load_queries(a, sp, head, rg * kRows);
-    run(a, s, head, cols, i0, i1, min_pos, max_pos);
+    run(a, sp, s, head, rg * kRows, cols, i0, i1, min_pos, max_pos);
     finish(a, sp, head, rg * kRows, piece_o, piece_ml);
   }
 };
@@ -493,10 +474,10 @@ __device__ __forceinline__ GroupRange group_range(const Rows::Span &sp, int grou
 
 // WHOLE: a block per (sequence, head, row group), for calls whose items are all short.  Otherwise all
 // items' columns, in order, in equal pieces.
-template <typename QT, int D, int MT, bool WHOLE>
-__global__ void __launch_bounds__(kTokenWarps * 32, (D == 64 && MT == 1 ? 3 : 2))
+template <typename QT, int D, int RB, bool WHOLE>
+__global__ void __launch_bounds__(kTokenWarps * 32, (RB == 1 ? (D == 64 && sizeof(QT) == 2 ? 4 : 3) : RB == 2 && D == 64 ? 3 : 2))
     attend_tokens(Call<QT> a, int groups, Pieces pieces) {
-  using K = TokenKernel<QT, D, MT>;
+  using K = TokenKernel<QT, D, RB>;
   pdl_prologue();
   K k;
   const int heads = a.cache.n_kv_heads;
@@ -603,9 +584,9 @@ __global__ void __launch_bounds__(kTokenWarps * 32, (D == 64 && MT == 1 ? 3 : 2)
 }
 
 // One item that was cut: block blockIdx.x has its first piece, the blocks after it the others.
-template <typename QT, int D, int MT>
+template <typename QT, int D, int RB>
 __global__ void __launch_bounds__(128) merge_pieces(Call<QT> a, Pieces pieces) {
-  constexpr int kRows = 16 * MT;
+  constexpr int kRows = 8 * RB;
   pdl_prologue();
   const int4 it = pieces.first[blockIdx.x];
   if (it.x < 0)
@@ -725,13 +706,13 @@ __global__ void __launch_bounds__(128)
 constexpr int kMostBlocksPerSm = 4;
 
 // Blocks of attend_tokens on the current device; the workspace is laid out for this many.
-template <typename QT, int D, int MT> int token_grid() {
-  const int per_sm = blocks_per_sm_smem(attend_tokens<QT, D, MT, false>, kTokenWarps * 32, TokenKernel<QT, D, MT>::kSmem);
+template <typename QT, int D, int RB> int token_grid() {
+  const int per_sm = blocks_per_sm_smem(attend_tokens<QT, D, RB, false>, kTokenWarps * 32, TokenKernel<QT, D, RB>::kSmem);
   return sm_count() * std::min(std::max(per_sm, 1), kMostBlocksPerSm);
 }
-template <typename QT, int D, int MT>
+template <typename QT, int D, int RB>
 void launch_tokens(cudaStream_t stream, const Call<QT> &a, void *workspace) {
-  using K = TokenKernel<QT, D, MT>;
+  using K = TokenKernel<QT, D, RB>;
   const int heads = a.cache.n_kv_heads;
   const long most_rows = std::min((long)a.rows.max_new * a.group, (long)kMaxTokenRows);
   const int groups = (int)((most_rows + K::kRows - 1) / K::kRows);
@@ -742,23 +723,26 @@ void launch_tokens(cudaStream_t stream, const Call<QT> &a, void *workspace) {
                              (long)a.rows.pages_stride);
   const dim3 block(kTokenWarps * 32);
   if (most <= 2 * kMinPages && items <= 0x7fffffff) {
-    blocks_per_sm_smem(attend_tokens<QT, D, MT, true>, kTokenWarps * 32, K::kSmem);
-    launch_kernel(attend_tokens<QT, D, MT, true>, dim3((unsigned)items), block, K::kSmem, stream, a, groups, Pieces{});
+    blocks_per_sm_smem(attend_tokens<QT, D, RB, true>, kTokenWarps * 32, K::kSmem);
+    launch_kernel(attend_tokens<QT, D, RB, true>, dim3((unsigned)items), block, K::kSmem, stream, a, groups, Pieces{});
     return;
   }
-  const int grid = (int)std::min((long)token_grid<QT, D, MT>(), items * most);
+  const int grid = (int)std::min((long)token_grid<QT, D, RB>(), items * most);
   const Pieces pieces = Pieces::at(workspace, grid, K::kRows, D);
-  launch_kernel(attend_tokens<QT, D, MT, false>, dim3(grid), block, K::kSmem, stream, a, groups, pieces);
+  launch_kernel(attend_tokens<QT, D, RB, false>, dim3(grid), block, K::kSmem, stream, a, groups, pieces);
   const PdlScope chained(GPTOSS_PDL);
-  launch_kernel(merge_pieces<QT, D, MT>, dim3(grid, K::kRows * D / 4 / 128), dim3(128), 0, stream, a, pieces);
+  launch_kernel(merge_pieces<QT, D, RB>, dim3(grid, K::kRows * D / 4 / 128), dim3(128), 0, stream, a, pieces);
 }
 
 template <typename QT, int D> void launch(cudaStream_t stream, const Call<QT> &a, void *workspace) {
-  if ((long)a.rows.max_new * a.group <= 16)
+  const long rows = (long)a.rows.max_new * a.group;
+  if (rows <= 8)
     launch_tokens<QT, D, 1>(stream, a, workspace);
-  else
+  else if (rows <= 16)
     launch_tokens<QT, D, 2>(stream, a, workspace);
-  if ((long)a.rows.max_new * a.group > kMaxTokenRows)
+  else
+    launch_tokens<QT, D, 4>(stream, a, workspace);
+  if (rows > kMaxTokenRows)
     launch_kernel(attend_rows<QT, D>, dim3(a.rows.T, (a.n_q_heads + 3) / 4), dim3(128), 0, stream, a);
 }
 

@@ -47,6 +47,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// An 8x8 matrix of 16-bit values (lane: row g, columns 2t, 2t + 1) transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
 // Exponent field of a power-of-two scale; 0 for 0.
 __device__ __forceinline__ int exponent_field(float s) { return (int)(__float_as_uint(s) >> 23) & 0xff; }
 __device__ __forceinline__ float two_to(int e) { // e in [-126, 127]; below: 0
