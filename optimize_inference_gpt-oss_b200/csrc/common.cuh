@@ -267,6 +267,26 @@ __device__ __forceinline__ bool mbar_wait(void *bar, uint32_t parity) {
       return false;
   }
 }
+// The same by shared-space address, looking once before it starts to count.
+__device__ __forceinline__ bool mbar_try_at(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+               "selp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done)
+               : "r"(bar), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool mbar_wait_at(uint32_t bar, uint32_t parity) {
+  if (mbar_try_at(bar, parity))
+    return true;
+  const long long t0 = clock64();
+  while (!mbar_try_at(bar, parity))
+    if (clock64() - t0 > kWaitCycles)
+      return false;
+  return true;
+}
 __device__ __forceinline__ void bulk_load(void *smem_dst, const void *gmem_src, uint32_t bytes, void *bar) {
   asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                    smem_u32(smem_dst)),

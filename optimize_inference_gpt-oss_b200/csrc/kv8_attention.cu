@@ -6,10 +6,12 @@
 // are the 16-row tiles of a matrix instruction; one pass over the pages with the running maximum and
 // sum of each row.  What bounds it is the cache's bytes: at 16 rows or fewer a token costs one byte per
 // element and some twelve instructions per 4 bytes.  So:
-//   - a warp works alone on steps of CH tokens, its loads going from global memory straight into the
-//     registers that feed the matrix instruction (the order of a head's elements within a product and
-//     of a step's tokens is free, and is chosen so that a lane needs 16 or 8 consecutive bytes), the
-//     next step's loads in flight while this one is computed; no shared memory, no barrier per step;
+//   - a warp works alone on steps of CH tokens: one lane asks the copy engine for the keys and the values of
+//     the steps to come (cp.async.bulk, 2-4 KB each, a page's keys or values of a head being consecutive) into
+//     the warp's own 16 KB ring, each part with its own barrier, so that 12 to 16 KB per warp are in flight
+//     at any time and the block meets only at the end;
+//   - the order of a head's elements within a product and of a step's tokens is free, and is chosen so
+//     that a lane needs 16 or 8 consecutive bytes of a token;
 //   - codes become fp16 exactly (kv8_mma.cuh); key scales multiply the scores, value scales, powers
 //     of two, multiply the codes relative to the largest met so far;
 //   - queries are brought to fp16 range by a power of two per row; a bf16 row is then exact, an fp32 row
@@ -31,6 +33,9 @@ constexpr int kWeightBits = 9, kValueBits = 5;
 constexpr int kTokenWarps = 4;
 constexpr int kMaxTokenRows = 64; // (new tokens) x (query heads per key/value head) of one sequence
 constexpr int kMinPages = 8;      // of a block's piece: below that joining costs more than it saves
+// What starting and ending an item costs a block, in pages (some 3 us where a page takes 0.6): without it a
+// block that got many short sequences ran 130 us where the others took 90.
+constexpr int kItemPages = 5;
 
 template <typename QT> struct Call {
   Layer cache;
@@ -43,6 +48,7 @@ template <typename QT> struct Call {
   const float *sinks;
   void *out;
   long out_row_stride;
+  unsigned *giveups;
   bool out_f32, q_vec, out_vec; // vec: rows may be read / written 4 elements at a time
 };
 
@@ -81,9 +87,10 @@ __device__ __forceinline__ void value_factor(int e, uint32_t &mul, uint32_t &add
   mul = m * 0x10001u, add = a * 0x10001u;
 }
 
-// Row n of an 8-token tile of scores holds this token of the tile: the tokens whose values the lanes
-// of a quad load together are then neighbours (256 consecutive bytes per load).
-__device__ __forceinline__ int token_of(int n) { return (n >> 1) + 4 * (n & 1); }
+// Row n of an 8-token tile of scores holds this token of the tile (the lowest bit flipped in every
+// other pair): neighbouring rows and the rows of a quad's lanes then fall into both halves of the 128
+// bytes that shared memory's banks repeat over.
+__device__ __forceinline__ int token_of(int n) { return n ^ ((n >> 1) & 1); }
 
 template <typename QT> __device__ __forceinline__ void load4(const QT *p, bool vec, float (&v)[4]) {
   if (vec) {
@@ -126,39 +133,35 @@ template <typename QT, int D, int RB> struct TokenKernel {
   static constexpr int TT = CH / 16, KS = D / 16, DT = D / 16;        // 16-token tiles, products of a score, 16-element tiles
   static constexpr int kRows = 8 * RB;
   static constexpr int kPitch = D + 4; // floats of a row in shared memory
-  static constexpr int kSmem = kTokenWarps * kRows * (kPitch * 4 + 8);
+  static constexpr int kPart = CH * D;              // bytes of a step's keys, and of its values
+  static constexpr int kDepth = 8192 / kPart;       // steps' keys (and values) in a warp's ring
+  static constexpr int kResult = kRows * (kPitch * 4 + 8); // a warp's results, which lie where its ring was
+  static constexpr int kRing = 2 * kDepth * kPart > kResult ? 2 * kDepth * kPart : kResult; // 16 KB per warp
+  static constexpr int kSmem = kTokenWarps * (kRing + 2 * kDepth * 8 + kDepth * 16);
   using VWord = typename std::conditional<D == 64, uint2, uint4>::type;
 
-  uint4 K[TT][2][D / 64]; // [tile][token g / g + 8]
-  VWord V[TT][4];         // [tile][the four tokens of a lane]
   uint32_t q[RB][KS][2], q_rest[kSplit ? RB : 1][kSplit ? KS : 1][2];
   float row_factor[RB][2], m[RB][2], l[RB][2], o[RB][DT][4]; // of rows 2t, 2t + 1 of each 8
   int row_pos[RB][2];                                        // -1: no such row
   int value_exp;
+  uint32_t ring, bars; // this warp's, as shared-space addresses
+  int4 *slots;         // what a part is: page, step, scales
+  int done;            // parts used so far, over all items
+  bool lost;           // a copy did not arrive in time
 
-  __device__ __forceinline__ void load_keys(const int8_t *block, int step) {
-    const int lane = threadIdx.x & 31, n = token_of(lane >> 2), t = lane & 3;
-#pragma unroll
-    for (int i = 0; i < TT; i++)
-#pragma unroll
-      for (int half = 0; half < 2; half++)
-#pragma unroll
-        for (int j = 0; j < D / 64; j++)
-          K[i][half][j] = ld_stream(block + (size_t)(step * CH + 16 * i + 8 * half + n) * D + j * 64 + t * 16);
-  }
-  __device__ __forceinline__ void load_values(const int8_t *block, int step) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int i = 0; i < TT; i++)
-#pragma unroll
-      for (int c = 0; c < 4; c++) { // rows 2t, 2t + 1, 2t + 8, 2t + 9 of the tile
-        const int token = step * CH + 16 * i + 8 * (c >> 1) + token_of(2 * t + (c & 1));
-        const int8_t *p = block + (size_t)(kPage + token) * D + g * (D / 8);
-        if constexpr (D == 64)
-          asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(V[i][c].x), "=r"(V[i][c].y) : "l"(p));
-        else
-          V[i][c] = ld_stream(p);
-      }
+  __device__ __forceinline__ void setup() {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int warp = threadIdx.x >> 5;
+    ring = smem_u32(smem) + warp * kRing;
+    bars = smem_u32(smem) + kTokenWarps * kRing + warp * 2 * kDepth * 8;
+    slots = reinterpret_cast<int4 *>(smem + kTokenWarps * (kRing + 2 * kDepth * 8)) + warp * kDepth;
+    done = 0, lost = false;
+    if ((threadIdx.x & 31) == 0) {
+      for (int i = 0; i < 2 * kDepth; i++)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + i * 8) : "memory");
+      mbar_init_fence();
+    }
+    __syncwarp();
   }
 
   // The group's queries as right operands (lane: row g), a row's elements in the order that K's lanes
@@ -223,15 +226,23 @@ template <typename QT, int D, int RB> struct TokenKernel {
       }
   }
 
-  __device__ __forceinline__ void scores(float (&s)[RB][TT][4]) {
+  __device__ __forceinline__ void scores(float (&s)[RB][TT][4], uint32_t keys) {
+    const int lane = threadIdx.x & 31;
+    keys += token_of(lane >> 2) * D + (lane & 3) * 16;
 #pragma unroll
     for (int i = 0; i < TT; i++) {
+      uint4 K[2][D / 64]; // tokens g and g + 8 of the tile
+#pragma unroll
+      for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int j = 0; j < D / 64; j++)
+          K[half][j] = lds16(keys + (16 * i + 8 * half) * D + j * 64);
 #pragma unroll
       for (int b = 0; b < RB; b++)
         s[b][i][0] = s[b][i][1] = s[b][i][2] = s[b][i][3] = 0.0f;
 #pragma unroll
       for (int j = 0; j < KS; j++) {
-        const uint32_t u = biased(word(K[i][0][j / 4], j % 4)), v = biased(word(K[i][1][j / 4], j % 4));
+        const uint32_t u = biased(word(K[0][j / 4], j % 4)), v = biased(word(K[1][j / 4], j % 4));
         const uint32_t k[4] = {minus_1152(low_pair(u)), minus_1152(low_pair(v)), minus_1152(high_pair(u)),
                                minus_1152(high_pair(v))};
 #pragma unroll
@@ -303,7 +314,9 @@ template <typename QT, int D, int RB> struct TokenKernel {
           o[b][j][0] *= fade[b][0], o[b][j][1] *= fade[b][1], o[b][j][2] *= fade[b][0], o[b][j][3] *= fade[b][1];
   }
 
-  __device__ __forceinline__ void add_values(const float (&s)[RB][TT][4], int v_exp) {
+  __device__ __forceinline__ void add_values(const float (&s)[RB][TT][4], int v_exp, uint32_t values) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    const uint32_t even = values + token_of(2 * t) * D + (lane >> 2) * (D / 8), odd = values + token_of(2 * t + 1) * D + (lane >> 2) * (D / 8);
     uint32_t mul, add;
     value_factor(v_exp == 0 ? -99 : v_exp - value_exp + kValueBits, mul, add);
 #pragma unroll
@@ -318,12 +331,16 @@ template <typename QT, int D, int RB> struct TokenKernel {
           if constexpr (kSplit)
             rest[b][half] = transposed(pack_rest(w, s[b][i][2 * half], s[b][i][2 * half + 1]));
         }
+      VWord V[4]; // of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of the tile
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        load_word(V[c], (c & 1 ? odd : even) + (16 * i + 8 * (c >> 1)) * D);
 #pragma unroll
       for (int w = 0; w < D / 32; w++) { // words of 4 elements: two 16-element tiles' rows g and g + 8
         uint32_t c[4];
 #pragma unroll
         for (int x = 0; x < 4; x++)
-          c[x] = biased(word(V[i][x], w));
+          c[x] = biased(word(V[x], w));
 #pragma unroll
         for (int hi = 0; hi < 2; hi++) {
           const uint32_t x = __byte_perm(c[0], c[1], hi ? 0x7362 : 0x5140), y = __byte_perm(c[2], c[3], hi ? 0x7362 : 0x5140);
@@ -339,68 +356,112 @@ template <typename QT, int D, int RB> struct TokenKernel {
       }
     }
   }
+  static __device__ __forceinline__ void load_word(uint4 &v, uint32_t a) { v = lds16(a); }
+  static __device__ __forceinline__ void load_word(uint2 &v, uint32_t a) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  }
   static __device__ __forceinline__ uint32_t word(uint2 v, int w) { return w ? v.y : v.x; }
   static __device__ __forceinline__ uint32_t word(uint4 v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
+
+  // Part p of the warp's sequence of keys (kind 0) or values (kind 1): where it lies, its barrier.
+  __device__ __forceinline__ uint32_t part_at(int p, int kind) const { return ring + (2 * (p % kDepth) + kind) * kPart; }
+  __device__ __forceinline__ uint32_t bar_at(int p, int kind) const { return bars + (2 * (p % kDepth) + kind) * 8; }
+  // One lane asks the copy engine for a part; its barrier completes when the bytes are there.
+  __device__ __forceinline__ void start(int p, int kind, const int8_t *block, int step) const {
+    const uint32_t bar = bar_at(p, kind);
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kPart) : "memory");
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(part_at(p, kind)),
+                 "l"(block + (size_t)(kind * kPage + step * CH) * D), "r"(kPart), "r"(bar)
+                 : "memory");
+  }
+  __device__ __forceinline__ bool arrived(int p, int kind) const { return mbar_wait_at(bar_at(p, kind), p / kDepth & 1); }
 
   // The columns [i0, i1) of an item, steps dealt to the block's warps in turn.
   __device__ __forceinline__ void run(const Call<QT> &a, const Rows::Span &sp, int s, int head, int row0, const Columns &cols,
                                       int i0, int i1, int min_pos, int max_pos) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int end = i1 * kSteps;
+    const int j0 = i0 * kSteps + warp, end = i1 * kSteps;
+    const int steps = j0 < end && !lost ? (end - j0 + kTokenWarps - 1) / kTokenWarps : 0;
     const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
-    int page_of = -1, held = i0 * kSteps + warp; // lane l has the page of step held + 4 l
+    int page_of = -1, held = -32, ahead = 0; // lane l has the page and scales of step held + l; steps before `ahead` are asked for
     float2 scale_of = make_float2(0.0f, 0.0f);
-    auto fetch = [&]() {
-      const int j = held + kTokenWarps * lane;
-      page_of = j < end ? a.cache.checked(__ldg(table + cols.at(j / kSteps))) : -1;
-      if (page_of >= 0)
-        scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
+    int asked = done; // parts
+    auto ask_keys = [&]() { // of the next step that has a page
+      for (; ahead < steps; ahead = held + 32) {
+        if (ahead >= held + 32) {
+          held += 32;
+          const int j = j0 + kTokenWarps * (held + lane);
+          page_of = j < end ? a.cache.checked(__ldg(table + cols.at(j / kSteps))) : -1;
+          if (page_of >= 0)
+            scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, page_of >= 0) >> (ahead - held);
+        if (there) {
+          ahead += __ffs(there) - 1;
+          const int page = __shfl_sync(0xffffffffu, page_of, ahead - held);
+          const float ks = __shfl_sync(0xffffffffu, scale_of.x, ahead - held), vs = __shfl_sync(0xffffffffu, scale_of.y, ahead - held);
+          if (lane == 0) {
+            slots[asked % kDepth] = make_int4(page, j0 + kTokenWarps * ahead, __float_as_int(ks), __float_as_int(vs));
+            start(asked, 0, a.cache.template block<D>(page, head), (j0 + kTokenWarps * ahead) % kSteps);
+          }
+          asked++, ahead++;
+          return;
+        }
+      }
+    };
+    auto ask_values = [&](int p) {
+      if (p < asked && lane == 0) {
+        const int4 it = slots[p % kDepth];
+        start(p, 1, a.cache.template block<D>(it.x, head), it.y % kSteps);
+      }
     };
     begin();
-    int j = held, at = 0, page = -1;
-    if (j < end) {
-      fetch();
-      page = __shfl_sync(0xffffffffu, page_of, 0);
-      if (page >= 0) {
-        load_keys(a.cache.template block<D>(page, head), j % kSteps);
-        load_values(a.cache.template block<D>(page, head), j % kSteps);
-      }
+#pragma unroll 1
+    for (int d = 0; d < kDepth; d++) {
+      ask_keys();
+      ask_values(done + d);
     }
-    load_queries(a, sp, head, row0); // while the first step's loads are on their way
-    float ks = __shfl_sync(0xffffffffu, scale_of.x, 0), vs = __shfl_sync(0xffffffffu, scale_of.y, 0);
-    for (; j < end; j += kTokenWarps) {
-      if (++at == 32) {
-        held += 32 * kTokenWarps, at = 0;
-        fetch();
+    load_queries(a, sp, head, row0); // while the first parts are on their way
+#pragma unroll 1
+    for (; done < asked; done++) {
+      __syncwarp();
+      const int4 it = slots[done % kDepth];
+      if (!arrived(done, 0)) {
+        lost = true;
+        break;
       }
-      const int next = __shfl_sync(0xffffffffu, page_of, at), next_step = (j + kTokenWarps) % kSteps;
-      const float next_ks = __shfl_sync(0xffffffffu, scale_of.x, at), next_vs = __shfl_sync(0xffffffffu, scale_of.y, at);
-      const int8_t *next_block = a.cache.template block<D>(max(next, 0), head);
       float w[RB][TT][4];
-      if (page >= 0)
-        scores(w);
-      if (next >= 0)
-        load_keys(next_block, next_step);
-      if (page >= 0) {
-        const int token = cols.at(j / kSteps) * kPage + (j % kSteps) * CH, v_exp = exponent_field(vs);
-        if (token + CH - 1 <= min_pos && (a.window <= 0 || token > max_pos - a.window || token + CH <= a.n_first))
-          weigh<false>(w, ks, v_exp, token, a.window, a.n_first);
-        else
-          weigh<true>(w, ks, v_exp, token, a.window, a.n_first);
-        add_values(w, v_exp);
+      scores(w, part_at(done, 0));
+      __syncwarp(); // every lane has read the keys and the slot
+      ask_keys();
+      const int token = cols.at(it.y / kSteps) * kPage + (it.y % kSteps) * CH, v_exp = exponent_field(__int_as_float(it.w));
+      if (token + CH - 1 <= min_pos && (a.window <= 0 || token > max_pos - a.window || token + CH <= a.n_first))
+        weigh<false>(w, __int_as_float(it.z), v_exp, token, a.window, a.n_first);
+      else
+        weigh<true>(w, __int_as_float(it.z), v_exp, token, a.window, a.n_first);
+      if (!arrived(done, 1)) {
+        lost = true;
+        break;
       }
-      if (next >= 0)
-        load_values(next_block, next_step);
-      page = next, ks = next_ks, vs = next_vs;
+      add_values(w, v_exp, part_at(done, 1));
+      __syncwarp();
+      ask_values(done + kDepth);
+    }
+    if (lost && done < asked) { // counted; what is still on its way is waited for (again with a limit) before the block ends
+      if (lane == 0 && a.giveups)
+        atomicAdd(a.giveups, 1u);
+      for (int p = done; p < asked; p++)
+        arrived(p, 0), arrived(p, 1);
+      done = asked;
     }
   }
 
   // The warps' results joined: into the output, or into a piece for merge_pieces.  Whole block.
   __device__ __forceinline__ void finish(const Call<QT> &a, const Rows::Span &sp, int head, int row0, float *piece_o,
                                          float2 *piece_ml) {
-    extern __shared__ float4 smem4[];
-    float *so = reinterpret_cast<float *>(smem4);
-    float2 *sml = reinterpret_cast<float2 *>(so + kTokenWarps * kRows * kPitch);
+    extern __shared__ __align__(16) uint8_t smem[];
+    auto so = [&](int w, int r) { return reinterpret_cast<float *>(smem + w * kRing) + r * kPitch; };
+    auto sml = [&](int w) { return reinterpret_cast<float2 *>(smem + w * kRing + kRows * kPitch * 4); };
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const float unit = two_to(value_exp - 127 - kValueBits);
 #pragma unroll
@@ -413,9 +474,9 @@ template <typename QT, int D, int RB> struct TokenKernel {
           sum += __shfl_xor_sync(0xffffffffu, sum, x);
         const int r = 8 * b + 2 * t + e;
         if (g == 0)
-          sml[warp * kRows + r] = make_float2(m[b][e], sum * two_to(-kWeightBits));
+          sml(warp)[r] = make_float2(m[b][e], sum * two_to(-kWeightBits));
         const float f = sum > 0.0f ? unit / sum : 0.0f;
-        float *row = so + (warp * kRows + r) * kPitch + g * (D / 8);
+        float *row = so(warp, r) + g * (D / 8);
 #pragma unroll
         for (int j = 0; j < DT; j += 2)
           *reinterpret_cast<float4 *>(row + 2 * j) =
@@ -431,14 +492,14 @@ template <typename QT, int D, int RB> struct TokenKernel {
       float top = z, sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < kTokenWarps; w++) {
-        ml[w] = sml[w * kRows + r];
+        ml[w] = sml(w)[r];
         top = fmaxf(top, ml[w].x);
       }
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kTokenWarps; w++) {
         const float part = ml[w].y != 0.0f ? ml[w].y * fast_exp2(ml[w].x - top) : 0.0f; // a NaN passes
-        const float4 x = *reinterpret_cast<const float4 *>(so + (w * kRows + r) * kPitch + d);
+        const float4 x = *reinterpret_cast<const float4 *>(so(w, r) + d);
         sum += part;
         acc.x += part * x.x, acc.y += part * x.y, acc.z += part * x.z, acc.w += part * x.w;
       }
@@ -455,7 +516,8 @@ template <typename QT, int D, int RB> struct TokenKernel {
         store4(a, (size_t)row * a.out_row_stride + (size_t)h * D + d, acc);
       }
     }
-    __syncthreads(); // the arrays may be used for the next item
+    fence_async_smem();
+    __syncthreads(); // the rings may be written by the copy engine again
   }
 
   __device__ __forceinline__ void item(const Call<QT> &a, const Rows::Span &sp, int s, int head, int rg, const Columns &cols,
@@ -475,11 +537,12 @@ __device__ __forceinline__ GroupRange group_range(const Rows::Span &sp, int grou
 // WHOLE: a block per (sequence, head, row group), for calls whose items are all short.  Otherwise all
 // items' columns, in order, in equal pieces.
 template <typename QT, int D, int RB, bool WHOLE>
-__global__ void __launch_bounds__(kTokenWarps * 32, (RB == 1 ? (D == 64 && sizeof(QT) == 2 ? 4 : 3) : RB == 2 && D == 64 ? 3 : 2))
+__global__ void __launch_bounds__(kTokenWarps * 32, RB <= 2 ? 3 : 2)
     attend_tokens(Call<QT> a, int groups, Pieces pieces) {
   using K = TokenKernel<QT, D, RB>;
   pdl_prologue();
   K k;
+  k.setup();
   const int heads = a.cache.n_kv_heads;
   auto n_groups = [&](const Rows::Span &sp) {
     const long R = (long)sp.q * a.group;
@@ -494,12 +557,12 @@ __global__ void __launch_bounds__(kTokenWarps * 32, (RB == 1 ? (D == 64 && sizeo
     const Columns cols = columns(a.rows, a.window, a.n_first, gr.lo, gr.hi);
     k.item(a, sp, s, head, rg, cols, 0, cols.n, gr.lo, gr.hi, nullptr, nullptr);
   } else {
-    // columns of a sequence and one head
+    // work of a sequence and one head: its items' columns and kItemPages for each item
     auto cost = [&](const Rows::Span &sp) {
       int n = 0;
       for (int rg = 0; rg < n_groups(sp); rg++) {
         const GroupRange gr = group_range(sp, a.group, rg, K::kRows);
-        n += columns(a.rows, a.window, a.n_first, gr.lo, gr.hi).n;
+        n += columns(a.rows, a.window, a.n_first, gr.lo, gr.hi).n + kItemPages;
       }
       return n;
     };
@@ -561,16 +624,18 @@ __global__ void __launch_bounds__(kTokenWarps * 32, (RB == 1 ? (D == 64 && sizeo
           for (int rg = 0; rg < groups_here && w < w_end; rg++) {
             const GroupRange gr = group_range(sp, a.group, rg, K::kRows);
             const Columns cols = columns(a.rows, a.window, a.n_first, gr.lo, gr.hi);
-            const long item1 = item0 + cols.n;
+            const long item1 = item0 + kItemPages + cols.n; // its columns are the last part of [item0, item1)
             if (w < item1) {
-              const int i0 = (int)(w - item0), i1 = (int)(min(item1, w_end) - item0);
-              const bool whole = i0 == 0 && i1 == cols.n;
-              const size_t slot = (size_t)blockIdx.x * 2 + (i0 == 0);
-              k.item(a, sp, s, head, rg, cols, i0, i1, gr.lo, gr.hi, whole ? nullptr : pieces.o + slot * K::kRows * D,
-                     whole ? nullptr : pieces.ml + slot * K::kRows);
-              if (i0 == 0 && !whole)
-                first = make_int4(s, head, rg, (int)((item1 - 1) / per));
-              w = item0 + i1;
+              const int i0 = max((int)(w - item0) - kItemPages, 0), i1 = (int)(min(item1, w_end) - item0) - kItemPages;
+              if (i0 < i1) {
+                const bool whole = i0 == 0 && i1 == cols.n;
+                const size_t slot = (size_t)blockIdx.x * 2 + (i0 == 0);
+                k.item(a, sp, s, head, rg, cols, i0, i1, gr.lo, gr.hi, whole ? nullptr : pieces.o + slot * K::kRows * D,
+                       whole ? nullptr : pieces.ml + slot * K::kRows);
+                if (i0 == 0 && !whole)
+                  first = make_int4(s, head, rg, (int)((item1 - 1) / per));
+              }
+              w = min(item1, w_end);
             }
             item0 = item1;
           }
@@ -583,36 +648,52 @@ __global__ void __launch_bounds__(kTokenWarps * 32, (RB == 1 ? (D == 64 && sizeo
   }
 }
 
-// One item that was cut: block blockIdx.x has its first piece, the blocks after it the others.
-template <typename QT, int D, int RB>
-__global__ void __launch_bounds__(128) merge_pieces(Call<QT> a, Pieces pieces) {
-  constexpr int kRows = 8 * RB;
+// One item that was cut: block blockIdx.x has its first piece, the blocks after it the others.  Threads
+// share 8 rows' elements four at a time, and the pieces among themselves where that leaves threads over (one
+// long sequence may have fifty).
+constexpr int kMergeThreads = 512;
+template <typename QT, int D, int RB> __global__ void __launch_bounds__(kMergeThreads) merge_pieces(Call<QT> a, Pieces pieces) {
+  constexpr int kRows = 8 * RB, D4 = D / 4;
+  __shared__ float4 part_of[kMergeThreads];
+  __shared__ float sum_of[kMergeThreads];
   pdl_prologue();
   const int4 it = pieces.first[blockIdx.x];
   if (it.x < 0)
     return;
   const Rows::Span sp = a.rows.span(it.x);
-  const int R = min(sp.q * a.group - it.z * kRows, kRows);
-  const int i = blockIdx.y * 128 + threadIdx.x, r = i / (D / 4), d = (i % (D / 4)) * 4;
-  if (r >= R)
+  const int row0 = blockIdx.y * 8, R = min(min(sp.q * a.group - it.z * kRows, kRows) - row0, 8);
+  if (R <= 0)
     return;
+  const int n = R * D4, slices = kMergeThreads / n, slice = threadIdx.x / n, i = threadIdx.x % n;
+  const int r = row0 + i / D4, d = (i % D4) * 4;
+  const int row = it.z * kRows + r, h = it.y * a.group + row % a.group;
   auto slot = [&](int b) { return ((size_t)b * 2 + (b == (int)blockIdx.x)) * kRows + r; };
-  float top = -INFINITY, sum = 0.0f;
+  const float z = a.sinks ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY;
+  float top = z, sum = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
   for (int b = blockIdx.x; b <= it.w; b++)
     top = fmaxf(top, pieces.ml[slot(b)].x);
-  const int row = it.z * kRows + r, h = it.y * a.group + row % a.group;
-  if (a.sinks)
-    top = fmaxf(top, fminf(__ldg(a.sinks + h) * kLog2e, 3e38f));
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int b = blockIdx.x; b <= it.w; b++) {
-    const float2 ml = pieces.ml[slot(b)];
-    const float4 x = *reinterpret_cast<const float4 *>(pieces.o + slot(b) * D + d);
-    const float part = ml.y != 0.0f ? ml.y * fast_exp2(ml.x - top) : 0.0f;
-    sum += part;
-    acc.x += part * x.x, acc.y += part * x.y, acc.z += part * x.z, acc.w += part * x.w;
+  if (slice < slices)
+#pragma unroll 8
+    for (int b = blockIdx.x + slice; b <= it.w; b += slices) {
+      const float2 ml = pieces.ml[slot(b)];
+      const float4 x = *reinterpret_cast<const float4 *>(pieces.o + slot(b) * D + d);
+      const float part = ml.y != 0.0f ? ml.y * fast_exp2(ml.x - top) : 0.0f;
+      sum += part;
+      acc.x += part * x.x, acc.y += part * x.y, acc.z += part * x.z, acc.w += part * x.w;
+    }
+  part_of[threadIdx.x] = acc, sum_of[threadIdx.x] = sum;
+  __syncthreads();
+  if (slice != 0)
+    return;
+  for (int k = 1; k < slices; k++) {
+    const float4 x = part_of[k * n + i];
+    sum += sum_of[k * n + i];
+    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
   }
   if (sum != 0.0f && a.sinks)
-    sum += fast_exp2(fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) - top);
+    sum += fast_exp2(z - top);
   const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
   store4(a, (size_t)(sp.row + row / a.group) * a.out_row_stride + (size_t)h * D + d,
          make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
@@ -723,7 +804,7 @@ void launch_tokens(cudaStream_t stream, const Call<QT> &a, void *workspace) {
                              (long)a.rows.pages_stride);
   const dim3 block(kTokenWarps * 32);
   if (most <= 2 * kMinPages && items <= 0x7fffffff) {
-    blocks_per_sm_smem(attend_tokens<QT, D, RB, true>, kTokenWarps * 32, K::kSmem);
+    (void)blocks_per_sm_smem(attend_tokens<QT, D, RB, true>, kTokenWarps * 32, K::kSmem);
     launch_kernel(attend_tokens<QT, D, RB, true>, dim3((unsigned)items), block, K::kSmem, stream, a, groups, Pieces{});
     return;
   }
@@ -731,7 +812,7 @@ void launch_tokens(cudaStream_t stream, const Call<QT> &a, void *workspace) {
   const Pieces pieces = Pieces::at(workspace, grid, K::kRows, D);
   launch_kernel(attend_tokens<QT, D, RB, false>, dim3(grid), block, K::kSmem, stream, a, groups, pieces);
   const PdlScope chained(GPTOSS_PDL);
-  launch_kernel(merge_pieces<QT, D, RB>, dim3(grid, K::kRows * D / 4 / 128), dim3(128), 0, stream, a, pieces);
+  launch_kernel(merge_pieces<QT, D, RB>, dim3(grid, RB), dim3(kMergeThreads), 0, stream, a, pieces);
 }
 
 template <typename QT, int D> void launch(cudaStream_t stream, const Call<QT> &a, void *workspace) {
@@ -752,7 +833,7 @@ void launch(cudaStream_t stream, int D, const Layer &cache, const void *qkv, lon
             long out_row_stride, void *workspace) {
   const size_t q4 = 4 * sizeof(QT), out4 = 4 * dtype_size(out_dtype);
   const Call<QT> a = {cache, static_cast<const QT *>(qkv), row_stride, n_q_heads, n_q_heads / cache.n_kv_heads, rows, scale,
-                      window, n_first, sinks, out, out_row_stride, out_dtype == GPTOSS_F32,
+                      window, n_first, sinks, out, out_row_stride, wait_giveups_word(), out_dtype == GPTOSS_F32,
                       (reinterpret_cast<uintptr_t>(qkv) & (q4 - 1)) == 0 && row_stride % 4 == 0,
                       (reinterpret_cast<uintptr_t>(out) & (out4 - 1)) == 0 && out_row_stride % 4 == 0};
   if (!a.q_vec || !a.out_vec)
