@@ -22,35 +22,18 @@
 //     beside short ones, one sequence alone); a sequence cut across blocks is joined by merge_pieces.
 #include <algorithm>
 
-#include "kv8_mma.cuh"
+#include "kv8_attention.cuh"
 
 namespace gptoss {
 namespace kv8 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWeightBits = 9, kValueBits = 5;
+constexpr int kWeightBits = 9;
 constexpr int kTokenWarps = 4;
-constexpr int kMaxTokenRows = 64; // (new tokens) x (query heads per key/value head) of one sequence
 constexpr int kMinPages = 8;      // of a block's piece: below that joining costs more than it saves
 // What starting and ending an item costs a block, in pages (some 3 us where a page takes 0.6): without it a
 // block that got many short sequences ran 130 us where the others took 90.
 constexpr int kItemPages = 5;
-
-template <typename QT> struct Call {
-  Layer cache;
-  const QT *qkv;
-  long row_stride;
-  int n_q_heads, group;
-  Rows rows;
-  float scale;
-  int window, n_first;
-  const float *sinks;
-  void *out;
-  long out_row_stride;
-  unsigned *giveups;
-  bool out_f32, q_vec, out_vec; // vec: rows may be read / written 4 elements at a time
-};
 
 // A block's piece of an item (sequence, head, row group) that other blocks have pieces of.
 struct Pieces {
@@ -67,62 +50,10 @@ struct Pieces {
   }
 };
 
-// The table columns a row group looks at: the first `head` ones, then those from `lo` on; n in all (at
-// least one, so that every row is visited; what it must not see is masked).
-struct Columns {
-  int head, lo, n;
-  __device__ __forceinline__ int at(int i) const { return i < head ? i : lo + i - head; }
-};
-__device__ __forceinline__ Columns columns(const Rows &rows, int window, int n_first, int min_pos, int max_pos) {
-  const int last = min(max(max_pos, 0) / kPage, rows.pages_stride - 1);
-  const int lo = window > 0 ? min(max(min_pos - window + 1, 0) / kPage, last) : 0;
-  const int head = min((int)(((long)n_first + kPage - 1) / kPage), lo);
-  return Columns{head, lo, head + last - lo + 1};
-}
-
-// fp16 2^e and -1152 * 2^e, twice in a word; e <= 5, zero below fp16's range.
-__device__ __forceinline__ void value_factor(int e, uint32_t &mul, uint32_t &add) {
-  const uint32_t m = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
-  const uint32_t a = e >= -24 ? 0x8080u | (uint32_t)(e + 25) << 10 : 0u;
-  mul = m * 0x10001u, add = a * 0x10001u;
-}
-
 // Row n of an 8-token tile of scores holds this token of the tile (the lowest bit flipped in every
 // other pair): neighbouring rows and the rows of a quad's lanes then fall into both halves of the 128
 // bytes that shared memory's banks repeat over.
 __device__ __forceinline__ int token_of(int n) { return n ^ ((n >> 1) & 1); }
-
-template <typename QT> __device__ __forceinline__ void load4(const QT *p, bool vec, float (&v)[4]) {
-  if (vec) {
-    if constexpr (sizeof(QT) == 4) {
-      const float4 f = *reinterpret_cast<const float4 *>(p);
-      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2 *>(p);
-      v[0] = bf16_lo(u.x), v[1] = bf16_hi(u.x), v[2] = bf16_lo(u.y), v[3] = bf16_hi(u.y);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      v[i] = load1(p + i);
-  }
-}
-// Four elements of the output, from element `at` on.
-template <typename QT> __device__ __forceinline__ void store4(const Call<QT> &a, size_t at, float4 v) {
-  if (a.out_f32) {
-    float *p = static_cast<float *>(a.out) + at;
-    if (a.out_vec)
-      *reinterpret_cast<float4 *>(p) = v;
-    else
-      p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
-  } else {
-    uint16_t *p = static_cast<uint16_t *>(a.out) + at;
-    if (a.out_vec)
-      *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-    else
-      store1(p, v.x), store1(p + 1, v.y), store1(p + 2, v.z), store1(p + 3, v.w);
-  }
-}
 
 // Scores and outputs are kept transposed (tokens x rows, elements x rows): the 8-wide side of the
 // matrix instruction is the rows', so that 8 rows (a group of 8 query heads and one token) waste nothing.
@@ -699,91 +630,6 @@ template <typename QT, int D, int RB> __global__ void __launch_bounds__(kMergeTh
          make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
 }
 
-// One warp per (row, query head): the plainest form.  A lane takes every 32nd token for the
-// scores, then D / 32 elements of the output.
-template <typename QT, int D>
-__global__ void __launch_bounds__(128)
-    attend_rows(Call<QT> a) {
-  pdl_prologue();
-  const Layer &cache = a.cache;
-  const Rows &rows = a.rows;
-  const int n_q_heads = a.n_q_heads, window = a.window, n_first = a.n_first;
-  const float *sinks = a.sinks;
-  const float scale = a.scale;
-  __shared__ float q_of[4][D], p_of[4][kPage];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.y * 4 + warp, row = blockIdx.x;
-  if (h >= n_q_heads)
-    return;
-  const int s = rows.find(row, [&](int i) { return rows.start(i); });
-  const Rows::Span sp = rows.span(s);
-  if (row < sp.row || row >= sp.row + sp.q || (long)sp.q * (n_q_heads / cache.n_kv_heads) <= kMaxTokenRows)
-    return;
-  const int pos = sp.pos + row - sp.row, head = h / (n_q_heads / cache.n_kv_heads);
-  bool bad = false, seen = false;
-  for (int i = lane; i < D; i += 32) {
-    const float q = load1(a.qkv + (size_t)row * a.row_stride + (size_t)h * D + i);
-    bad = bad || !isfinite(q);
-    q_of[warp][i] = isfinite(q) ? q * scale : 0.0f;
-  }
-  bad = __any_sync(0xffffffffu, bad);
-  __syncwarp();
-  float m = sinks ? sinks[h] : -INFINITY, l = m > -INFINITY ? 1.0f : 0.0f, acc[D / 32] = {};
-  const int from = window > 0 ? pos - window + 1 : 0; // tokens >= from are in the window
-  for (int p = 0; p < rows.pages_stride && p * kPage <= pos; p++) {
-    if (p * kPage + kPage <= from && p * kPage >= n_first)
-      continue;
-    const int page = cache.checked(rows.pages[(size_t)s * rows.pages_stride + p]);
-    if (page < 0)
-      continue;
-    const int8_t *codes = cache.block<D>(page, head);
-    const float ks = cache.scale(page, head)[0], vs = cache.scale(page, head)[1];
-    float z[2], top = m;
-    for (int u = 0; u < 2; u++) {
-      const int t = p * kPage + lane + 32 * u;
-      z[u] = -INFINITY;
-      if (t <= pos && (t >= from || t < n_first)) {
-        float dot = 0.0f;
-        for (int i = 0; i < D; i++)
-          dot += q_of[warp][i] * codes[(lane + 32 * u) * D + i];
-        z[u] = dot * ks;
-        seen = true;
-      }
-      top = fmaxf(top, z[u]);
-    }
-    for (int o = 16; o > 0; o >>= 1)
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (top == -INFINITY)
-      continue;
-    const float fade = expf(m - top);
-    m = top;
-    float sum = 0.0f;
-    for (int u = 0; u < 2; u++) {
-      const float w = expf(z[u] - m);
-      sum += w;
-      p_of[warp][lane + 32 * u] = w * vs;
-    }
-    l = l * fade + warp_sum(sum);
-    __syncwarp();
-    for (int i = 0; i < D / 32; i++) {
-      float a = 0.0f;
-      for (int t = 0; t < kPage; t++)
-        a += p_of[warp][t] * codes[(kPage + t) * D + i * 32 + lane];
-      acc[i] = acc[i] * fade + a;
-    }
-    __syncwarp();
-  }
-  bad = __any_sync(0xffffffffu, seen) && bad;
-  for (int i = 0; i < D / 32; i++) {
-    const size_t at = (size_t)row * a.out_row_stride + (size_t)h * D + i * 32 + lane;
-    const float v = bad ? NAN : l > 0.0f ? acc[i] / l : 0.0f;
-    if (a.out_f32)
-      static_cast<float *>(a.out)[at] = v;
-    else
-      store1(static_cast<uint16_t *>(a.out) + at, v);
-  }
-}
-
 constexpr int kMostBlocksPerSm = 4;
 
 // Blocks of attend_tokens on the current device; the workspace is laid out for this many.
@@ -824,7 +670,7 @@ template <typename QT, int D> void launch(cudaStream_t stream, const Call<QT> &a
   else
     launch_tokens<QT, D, 4>(stream, a, workspace);
   if (rows > kMaxTokenRows)
-    launch_kernel(attend_rows<QT, D>, dim3(a.rows.T, (a.n_q_heads + 3) / 4), dim3(128), 0, stream, a);
+    launch_tiles(stream, a, D);
 }
 
 template <typename QT>
