@@ -19,6 +19,8 @@
 // and their weights in two parts with two products.
 // Every wait is bounded: one that runs out is counted, tells the block's other roles, and the block frees its
 // tensor memory and ends.
+#include <type_traits>
+
 #include "kv8_attention.cuh"
 
 namespace gptoss {
@@ -29,37 +31,73 @@ constexpr int kTile = 128, kTiles = 2, kTileThreads = 416;
 constexpr int kTileBits = 7, kRise = 8; // weights are at most 2^(kTileBits + kRise) < 65504
 constexpr int kMeta = 16;
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 __device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// Registers a thread of this warpgroup may use from here on.  The block starts with 13 x 32 x 128; the converting warps go
+// down to 72 (128 threads) before the softmax warps' 152 (256) are granted: 9216 + 38912, and 4096 of the issuing
+// warp, are 52224 of 53248.
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+// One arrival for a warp, after all its lanes.
+__device__ __forceinline__ void arrive_warp(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0)
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Shared-memory operand in the 128-byte swizzle: rows of 128 bytes in groups of 8 (1024 bytes).  For keys and
 // queries a row is 64 elements of one token and `other` is unused; for values, read across (a row is one step of
-// the product's inner index), `other` is the distance of the next 64 elements.
-__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t other) {
-  return (uint64_t)(address >> 4 & 0x3fff) | (uint64_t)(other >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-         (uint64_t)2 << 61;
-}
+// the product's inner index), `other` is the distance of the next 64 elements.  The low word alone has addresses:
+// operands are moved on by adding bytes / 16 to it.
+__device__ __forceinline__ uint32_t operand_low(uint32_t address, uint32_t other) { return (address >> 4 & 0x3fff) | other >> 4 << 16; }
+constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
 // fp16 x fp16 -> fp32, 128 x n; `across`: the right operand as values lie.
 __host__ __device__ constexpr uint32_t shape_of(int n, bool across) {
   return 1u << 4 | (across ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
 }
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-               "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+// Issued by the lane that has `leader` set.  The whole warp comes here, so that operands stay in uniform
+// registers: with one lane in a branch of its own, moving them there took 2400 clocks per page.
+__device__ __forceinline__ void mma_smem(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add, uint32_t leader) {
+  asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "mov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+               "r"(a), "r"(b), "r"(shape), "r"(add), "r"(leader), "r"(kOperandHigh)
                : "memory");
 }
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-               "r"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add, uint32_t leader) {
+  asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "mov.b64 b, {%2, %6};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+               "r"(a), "r"(b), "r"(shape), "r"(add), "r"(leader), "r"(kOperandHigh)
                : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t leader) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+               "r"(leader)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
 #define GPTOSS_R8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
 #define GPTOSS_W8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
@@ -83,7 +121,7 @@ __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.s
 
 template <typename QT, int D> struct TileKernel {
   static constexpr bool kSplit = sizeof(QT) == 4;
-  static constexpr int kKeyStages = kSplit && D == 128 ? 2 : 3, kValueStages = 2, kRawStages = kSplit && D == 128 ? 2 : 3;
+  static constexpr int kKeyStages = D == 64 ? 4 : kSplit ? 2 : 3, kValueStages = kKeyStages, kRawStages = D == 64 ? 4 : kSplit ? 2 : 3;
   static constexpr int kQueryBytes = kTile * D * 2;                    // of a tile and part
   static constexpr int kPageBytes = kPage * D * 2;                     // a page's keys or values as fp16
   static constexpr int kRawBytes = 2 * kPage * D;                      // a page's codes, keys then values
@@ -165,22 +203,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
   k.stop = reinterpret_cast<volatile int *>(smem + K::kStopAt);
   k.giveups = a.giveups;
   Meta *const meta = reinterpret_cast<Meta *>(smem + K::kMetaAt);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31; // the same for all lanes, and known to be
   if (threadIdx.x == 0) {
     auto init = [&](int first, int n, int arrivals) {
       for (int i = first; i < first + n; i++)
         mbar_init(smem + K::kBars + i * 8, arrivals);
     };
-    init(K::kQueryFull, 1, kTile * tiles);
+    init(K::kQueryFull, 1, 4 * tiles);
     init(K::kScoreFull, 4, 1);
-    init(K::kWeightFull, 4, kTile);
+    init(K::kWeightFull, 4, 4);
     init(K::kOutDone, 2, 1);
-    init(K::kKeyFull, K::kKeyStages, kTile);
+    init(K::kKeyFull, K::kKeyStages, 4);
     init(K::kKeyFree, K::kKeyStages, 1);
-    init(K::kValueFull, K::kValueStages, kTile);
+    init(K::kValueFull, K::kValueStages, 4);
     init(K::kValueFree, K::kValueStages, 1);
     init(K::kRawFull, K::kRawStages, 1);
-    init(K::kRawFree, K::kRawStages, kTile);
+    init(K::kRawFree, K::kRawStages, 4);
     init(K::kDrained, 1, 1);
     *k.stop = 0;
     mbar_init_fence();
@@ -198,6 +236,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
 
   if (warp < 8) {
     // ---- softmax: a thread per row ----------------------------------------------------
+    more_registers<152>();
     const int tile = warp >> 2, r = threadIdx.x & (kTile - 1);
     const uint32_t lanes = (uint32_t)(warp & 3) << 21; // this warp's 32 lanes of tensor memory
     if (tile < tiles) {
@@ -211,7 +250,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
         const QT *p = a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D;
         float top = 0.0f;
         bool odd = false;
-#pragma unroll 4
+#pragma unroll 16
         for (int c = 0; c < D; c += 4) {
           float v[4];
           load4(p + c, a.q_vec, v);
@@ -247,40 +286,35 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
             K::store16(to + K::kQueryBytes + K::swizzled(r, c, kTile), rest[0], rest[1], rest[2], rest[3]);
         }
         fence_async_smem();
-        arrive(k.bar(K::kQueryFull));
+        arrive_warp(k.bar(K::kQueryFull));
       }
       float m = -INFINITY, l = 0.0f;
       int value_exp = 0, j = 0;
-      bool ok = true;
-      for (;; j++) {
-        if (!(ok = k.wait_warp(K::kScoreFull + tile * 2 + (j & 1), j >> 1 & 1)))
-          break;
-        tc_after_sync();
-        const Meta it = meta[j % kMeta];
-        if (it.token < 0)
-          break;
+      // Scores of page j to weights; false: the block is to end.
+      auto step = [&](auto masked, const Meta &it, int j) {
+        constexpr bool kMasked = decltype(masked)::value;
         uint32_t x[64];
         tmem_load32(scores_at(tile, j) + lanes, x);
         tmem_load32(scores_at(tile, j) + lanes + 32, x + 32);
         tmem_loaded();
-        const bool all = it.token + kPage - 1 <= min_pos &&
-                         (a.window <= 0 || it.token > max_pos - a.window || it.token + kPage <= a.n_first);
-        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-        float top = -INFINITY;
-        if (all) {
-#pragma unroll
-          for (int c = 0; c < kPage; c++)
-            top = fmaxf(top, __uint_as_float(x[c]));
-        } else {
+        uint32_t seen[2] = {0, 0};
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}; // four chains, so that none waits for itself
+        if constexpr (kMasked) {
           const int hi = pos - it.token, lo = a.window > 0 ? pos - a.window - it.token : -1, first = a.n_first - it.token;
-          seen[0] = seen[1] = 0;
 #pragma unroll
           for (int c = 0; c < kPage; c++) {
             const bool sees = c <= hi && (c > lo || c < first);
             seen[c >> 5] |= (uint32_t)sees << (c & 31);
-            top = fmaxf(top, sees ? __uint_as_float(x[c]) : -INFINITY);
+            tops[c & 3] = fmaxf(tops[c & 3], sees ? __uint_as_float(x[c]) : -INFINITY);
           }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kPage; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + 4 + e])));
         }
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const float f = row_factor * it.key_scale;
         const float now = top > -INFINITY ? fmaxf(m, top * f) : m;
         if (__any_sync(0xffffffffu, now > m + kRise || it.value_exp != value_exp)) {
@@ -290,8 +324,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
           l *= fade;
           value_exp = it.value_exp;
           if (j > 0) {
-            if (!(ok = k.wait_warp(K::kOutDone + tile, (j - 1) & 1)))
-              break;
+            if (!k.wait_warp(K::kOutDone + tile, (j - 1) & 1))
+              return false;
             tc_after_sync();
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -307,26 +341,43 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
         }
         const float off = (float)kTileBits - (m > -INFINITY ? m : 0.0f);
         uint32_t w[32];
-        float sum = 0.0f;
+        float2 sums[4] = {};
 #pragma unroll
         for (int c = 0; c < kPage; c += 2) {
-          float p0 = fast_exp2(fmaf(__uint_as_float(x[c]), f, off)), p1 = fast_exp2(fmaf(__uint_as_float(x[c + 1]), f, off));
-          if (!all) {
-            p0 = seen[c >> 5] >> (c & 31) & 1 ? p0 : 0.0f;
-            p1 = seen[c >> 5] >> ((c & 31) + 1) & 1 ? p1 : 0.0f;
+          const float2 z = fma2(make_float2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), make_float2(f, f), make_float2(off, off));
+          float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+          if constexpr (kMasked) {
+            p.x = seen[c >> 5] >> (c & 31) & 1 ? p.x : 0.0f;
+            p.y = seen[c >> 5] >> ((c & 31) + 1) & 1 ? p.y : 0.0f;
           }
-          sum += p0 + p1;
-          w[c / 2] = pack_f16(p0, p1);
+          sums[c / 2 & 3] = add2(sums[c / 2 & 3], p);
+          w[c / 2] = pack_f16(p.x, p.y);
           if constexpr (kSplit)
-            x[c / 2] = pack_rest(w[c / 2], p0, p1); // x[c / 2] has been read
+            x[c / 2] = pack_rest(w[c / 2], p.x, p.y); // x[c / 2] has been read
         }
-        l += sum;
+        const float2 sum = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
+        l += sum.x + sum.y;
         tmem_store32(scores_at(tile, j) + lanes, w);
         if constexpr (kSplit)
           tmem_store32(scores_at(tile, j) + lanes + 32, x);
+        return true;
+      };
+      bool ok = true;
+      for (;; j++) {
+        if (!(ok = k.wait_warp(K::kScoreFull + tile * 2 + (j & 1), j >> 1 & 1)))
+          break;
+        tc_after_sync();
+        const Meta it = meta[j % kMeta];
+        if (it.token < 0)
+          break;
+        const bool all = it.token + kPage - 1 <= min_pos &&
+                         (a.window <= 0 || it.token > max_pos - a.window || it.token + kPage <= a.n_first);
+        ok = all ? step(std::false_type{}, it, j) : step(std::true_type{}, it, j);
+        if (!ok)
+          break;
         tmem_stored();
         tc_before_sync();
-        arrive(k.bar(K::kWeightFull + tile * 2 + (j & 1)));
+        arrive_warp(k.bar(K::kWeightFull + tile * 2 + (j & 1)));
       }
       if (ok && j > 0)
         ok = k.wait_warp(K::kOutDone + tile, (j - 1) & 1);
@@ -360,6 +411,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
     }
   } else if (warp < 12) {
     // ---- codes to fp16 ------------------------------------------------------------------
+    fewer_registers<72>();
     const int t = threadIdx.x - 256, token = t >> 1, half = t & 1; // half of a token's codes
     const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
     int page_of = -1, held = -32, ahead = 0, asked = 0, value_exp = 0;
@@ -435,7 +487,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
           convert(from, k.base + K::kKeys + ks * K::kPageBytes, 0x3c003c00u, 0xe480e480u); // times 1, minus 1152
         }
         fence_async_smem();
-        arrive(k.bar(K::kKeyFull + ks));
+        arrive_warp(k.bar(K::kKeyFull + ks));
         if (!more)
           break;
         if (j >= K::kValueStages && !(ok = k.wait_warp(K::kValueFree + vs, (j / K::kValueStages - 1) & 1)))
@@ -444,8 +496,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
         value_factor(v_exp == 0 ? -99 : v_exp - value_exp + kValueBits, mul, add);
         convert(from + kPage * D, k.base + K::kValues + vs * K::kPageBytes, mul, add);
         fence_async_smem();
-        arrive(k.bar(K::kValueFull + vs));
-        arrive(k.bar(K::kRawFree + raw)); // this thread has read the raw stage
+        arrive_warp(k.bar(K::kValueFull + vs));
+        arrive_warp(k.bar(K::kRawFree + raw)); // this thread has read the raw stage
         used++;
         if (warp == 8 && !(ok = k.wait_warp(K::kRawFree + raw, j / K::kRawStages & 1)))
           break;
@@ -455,39 +507,43 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
     if (t == 0 && !ok) // what is still on its way is waited for, with a limit of its own
       for (int p = used; p < asked; p++)
         mbar_wait_at(k.bar(K::kRawFull + p % K::kRawStages), p / K::kRawStages & 1);
-  } else if (lane == 0) {
+  } else {
     // ---- matrix instructions --------------------------------------------------------------
     constexpr uint32_t kScoreShape = shape_of(kPage, false), kOutShape = shape_of(D, true);
-    auto score = [&](int tile, int j) {
-      const uint32_t q = k.base + K::kQueries + tile * (kSplit ? 2 : 1) * K::kQueryBytes;
-      const uint32_t keys = k.base + K::kKeys + (j % K::kKeyStages) * K::kPageBytes;
-#pragma unroll
-      for (int part = 0; part < (kSplit ? 2 : 1); part++)
-#pragma unroll
-        for (int i = 0; i < D / 16; i++)
-          mma_smem(scores_at(tile, j), operand(q + part * K::kQueryBytes + (i / 4) * kTile * 128 + (i % 4) * 32, 16),
-                   operand(keys + (i / 4) * kPage * 128 + (i % 4) * 32, 16), kScoreShape, part + i > 0);
-    };
-    bool ok = k.wait(K::kQueryFull, 0), more = true;
-    int n = 0; // pages whose scores have been asked for
+    const uint32_t leader = elected();
+    const uint32_t queries = operand_low(k.base + K::kQueries, 16), keys0 = operand_low(k.base + K::kKeys, 16),
+                   values0 = operand_low(k.base + K::kValues, kPage * 128);
+    bool ok = k.wait_warp(K::kQueryFull, 0), more = true;
+    int n = 0, key_stage = 0, value_stage = 0; // pages whose scores have been asked for; where the next ones lie
+    uint32_t key_turn = 0, value_turn = 0;
     // The scores of page n for `tile`; the page's keys are waited for with tile 0.
     auto next_scores = [&](int tile) {
       if (!more)
         return;
       if (tile == 0) {
-        if (!(ok = k.wait(K::kKeyFull + n % K::kKeyStages, n / K::kKeyStages & 1)))
+        if (!(ok = k.wait_warp(K::kKeyFull + key_stage, key_turn)))
           return;
         tc_after_sync();
       }
       const bool real = meta[n % kMeta].token >= 0;
-      if (real)
-        score(tile, n);
-      tc_commit(k.bar(K::kScoreFull + tile * 2 + (n & 1))); // also for the end of the pages
+      if (real) {
+        const uint32_t q = queries + tile * ((kSplit ? 2 : 1) * K::kQueryBytes / 16), keys = keys0 + key_stage * (K::kPageBytes / 16);
+#pragma unroll
+        for (int part = 0; part < (kSplit ? 2 : 1); part++)
+#pragma unroll
+          for (int i = 0; i < D / 16; i++)
+            mma_smem(scores_at(tile, n), q + (part * K::kQueryBytes + (i / 4) * kTile * 128 + (i % 4) * 32) / 16,
+                     keys + ((i / 4) * kPage * 128 + (i % 4) * 32) / 16, kScoreShape, part + i > 0, leader);
+      }
+      tc_commit(k.bar(K::kScoreFull + tile * 2 + (n & 1)), leader); // also for the end of the pages
       if (tile == tiles - 1) {
-        if (real)
-          tc_commit(k.bar(K::kKeyFree + n % K::kKeyStages));
+        if (real) {
+          tc_commit(k.bar(K::kKeyFree + key_stage), leader);
+          n++;
+          if (++key_stage == K::kKeyStages)
+            key_stage = 0, key_turn ^= 1;
+        }
         more = real;
-        n += real;
       }
     };
     for (int i = 0; i < 2 && ok; i++)
@@ -495,26 +551,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
         next_scores(tile);
     for (int j = 0; ok && j < n; j++) {
       for (int tile = 0; tile < tiles && ok; tile++) {
-        if (!(ok = k.wait(K::kWeightFull + tile * 2 + (j & 1), j >> 1 & 1)))
+        if (!(ok = k.wait_warp(K::kWeightFull + tile * 2 + (j & 1), j >> 1 & 1)))
           break;
-        if (tile == 0 && !(ok = k.wait(K::kValueFull + j % K::kValueStages, j / K::kValueStages & 1)))
+        if (tile == 0 && !(ok = k.wait_warp(K::kValueFull + value_stage, value_turn)))
           break;
         tc_after_sync();
-        const uint32_t values = k.base + K::kValues + (j % K::kValueStages) * K::kPageBytes;
+        const uint32_t values = values0 + value_stage * (K::kPageBytes / 16);
 #pragma unroll
         for (int part = 0; part < (kSplit ? 2 : 1); part++)
 #pragma unroll
           for (int i = 0; i < kPage / 16; i++)
-            mma_tmem(out_at(tile), scores_at(tile, j) + part * 32 + i * 8, operand(values + i * 2048, kPage * 128), kOutShape,
-                     j + part + i > 0);
-        tc_commit(k.bar(K::kOutDone + tile));
+            mma_tmem(out_at(tile), scores_at(tile, j) + part * 32 + i * 8, values + i * (2048 / 16), kOutShape, j + part + i > 0,
+                     leader);
+        tc_commit(k.bar(K::kOutDone + tile), leader);
         if (tile == tiles - 1)
-          tc_commit(k.bar(K::kValueFree + j % K::kValueStages));
+          tc_commit(k.bar(K::kValueFree + value_stage), leader);
         next_scores(tile);
       }
+      if (++value_stage == K::kValueStages)
+        value_stage = 0, value_turn ^= 1;
     }
     if (!ok) { // matrix instructions still running are waited for, with a limit, before their memory is given back
-      tc_commit(k.bar(K::kDrained));
+      tc_commit(k.bar(K::kDrained), leader);
       mbar_wait_at(k.bar(K::kDrained), 0);
     }
   }
