@@ -12,7 +12,8 @@
 //   - warps 0-3 and 4-7: softmax of tile 0 and 1.  A row's running maximum is raised only when the new one is
 //     2^8 above it, so that O is rescaled a few times per row and not once per page;
 //   - warps 8-11: codes (brought by the copy engine into a ring of raw pages) to fp16 in the 128-byte swizzled
-//     form the matrix instruction reads; once for both tiles;
+//     form the matrix instruction reads, once for both tiles; two warps for the keys and two for the values, since
+//     what a page costs them is mostly waiting (barriers, the fence before the matrix unit may read);
 //   - warp 12: one thread issues the matrix instructions.  Scores have two buffers per tile, so the next page's
 //     are ready when a softmax warp comes for them.
 // Queries, codes and weights are represented as in kv8_attention.cu: fp16, exact for codes and bf16 rows; fp32 rows
@@ -27,7 +28,7 @@ namespace gptoss {
 namespace kv8 {
 namespace {
 
-constexpr int kTile = 128, kTiles = 2, kTileThreads = 416;
+constexpr int kTile = 128;
 constexpr int kTileBits = 7, kRise = 8; // weights are at most 2^(kTileBits + kRise) < 65504
 constexpr int kMeta = 16;
 
@@ -55,11 +56,14 @@ __device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::a
 // warp, are 52224 of 53248.
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // One arrival for a warp, after all its lanes.
 __device__ __forceinline__ void arrive_warp(uint32_t bar) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0)
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+    arrive(bar);
 }
 
 // Shared-memory operand in the 128-byte swizzle: rows of 128 bytes in groups of 8 (1024 bytes).  For keys and
@@ -72,32 +76,40 @@ constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
 __host__ __device__ constexpr uint32_t shape_of(int n, bool across) {
   return 1u << 4 | (across ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
 }
-// Issued by the lane that has `leader` set.  The whole warp comes here, so that operands stay in uniform
-// registers: with one lane in a branch of its own, moving them there took 2400 clocks per page.
-__device__ __forceinline__ void mma_smem(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add, uint32_t leader) {
-  asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-               "mov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
-               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
-               "r"(a), "r"(b), "r"(shape), "r"(add), "r"(leader), "r"(kOperandHigh)
+// Four steps of 16 along the inner index, issued by one lane.  The whole warp comes here and elects it: operands
+// stay in uniform registers (with one lane in a branch of its own, moving them there took longer than the products).
+__device__ __forceinline__ void mma4_smem(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add) {
+  asm volatile("{\n\t.reg .pred p, q, t;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\telect.sync _|q, 0xffffffff;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+               "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+               "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+               "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+               "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t}" ::"r"(d),
+               "r"(a), "r"(b), "r"(shape), "r"(add), "r"(kOperandHigh)
                : "memory");
 }
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add, uint32_t leader) {
-  asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-               "mov.b64 b, {%2, %6};\n\t"
-               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
-               "r"(a), "r"(b), "r"(shape), "r"(add), "r"(leader), "r"(kOperandHigh)
+// `half`: columns from the first two steps' left operand to the others'.
+template <int half>
+__device__ __forceinline__ void mma4_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add) {
+  asm volatile("{\n\t.reg .pred p, q, t;\n\t.reg .b64 b;\n\t.reg .b32 x, y;\n\telect.sync _|q, 0xffffffff;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+               "mov.b64 b, {%2, %5};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
+               "add.u32 x, %1, 8;\n\tadd.u32 y, %2, 128;\n\tmov.b64 b, {y, %5};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, t;\n\t"
+               "add.u32 x, %1, %6;\n\tadd.u32 y, %2, 256;\n\tmov.b64 b, {y, %5};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, t;\n\t"
+               "add.u32 x, %1, %7;\n\tadd.u32 y, %2, 384;\n\tmov.b64 b, {y, %5};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, t;\n\t}" ::"r"(d),
+               "r"(a), "r"(b), "r"(shape), "r"(add), "r"(kOperandHigh), "n"(half), "n"(half + 8)
                : "memory");
 }
-__device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t leader) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
-               "r"(leader)
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
                : "memory");
-}
-__device__ __forceinline__ uint32_t elected() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r;
 }
 #define GPTOSS_R8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
 #define GPTOSS_W8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
@@ -114,23 +126,32 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *x) {
                GPTOSS_W8(x, 0), GPTOSS_W8(x, 8), GPTOSS_W8(x, 16), GPTOSS_W8(x, 24)
                : "memory");
 }
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t *x) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+               GPTOSS_W8(x, 0), GPTOSS_W8(x, 8)
+               : "memory");
+}
 #undef GPTOSS_R8
 #undef GPTOSS_W8
 __device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <typename QT, int D> struct TileKernel {
+template <typename QT, int D, int TILES> struct TileKernel {
   static constexpr bool kSplit = sizeof(QT) == 4;
+  static constexpr int kBuffers = TILES == 2 ? 2 : 1;                  // of scores, per tile
+  static constexpr int kConverters = 4 * TILES, kIssuer = kConverters + 4, kThreads = 32 * (kIssuer + 1);
+  static constexpr int kRowsOfBlock = kTile * TILES;
+  static_assert(TILES * (64 * kBuffers + D) <= 512, "tensor memory");
   static constexpr int kKeyStages = D == 64 ? 4 : kSplit ? 2 : 3, kValueStages = kKeyStages, kRawStages = D == 64 ? 4 : kSplit ? 2 : 3;
   static constexpr int kQueryBytes = kTile * D * 2;                    // of a tile and part
   static constexpr int kPageBytes = kPage * D * 2;                     // a page's keys or values as fp16
   static constexpr int kRawBytes = 2 * kPage * D;                      // a page's codes, keys then values
-  static constexpr int kQueries = 0, kKeys = kQueries + kTiles * (kSplit ? 2 : 1) * kQueryBytes;
+  static constexpr int kQueries = 0, kKeys = kQueries + TILES * (kSplit ? 2 : 1) * kQueryBytes;
   static constexpr int kValues = kKeys + kKeyStages * kPageBytes, kRaw = kValues + kValueStages * kPageBytes;
   static constexpr int kMetaAt = kRaw + kRawStages * kRawBytes, kBars = kMetaAt + kMeta * 16;
   // barriers
-  static constexpr int kQueryFull = 0, kScoreFull = 1 /* tile, buffer */, kWeightFull = kScoreFull + 4 /* tile, buffer */,
-                       kOutDone = kWeightFull + 4 /* tile */, kKeyFull = kOutDone + 2, kKeyFree = kKeyFull + kKeyStages,
+  static constexpr int kQueryFull = 0, kScoreFull = 1 /* tile, buffer */, kWeightFull = kScoreFull + TILES * kBuffers /* tile, buffer */,
+                       kOutDone = kWeightFull + TILES * kBuffers /* tile */, kKeyFull = kOutDone + TILES, kKeyFree = kKeyFull + kKeyStages,
                        kValueFull = kKeyFree + kKeyStages, kValueFree = kValueFull + kValueStages,
                        kRawFull = kValueFree + kValueStages, kRawFree = kRawFull + kRawStages, kDrained = kRawFree + kRawStages,
                        kBarCount = kDrained + 1;
@@ -179,23 +200,24 @@ struct Meta { // of a page: its first token (-1: there are no more), key scale, 
   int value_exp, unused;
 };
 
-template <typename QT, int D>
-__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
-  using K = TileKernel<QT, D>;
+template <typename QT, int D, int TILES>
+__global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT> a) {
+  using K = TileKernel<QT, D, TILES>;
   constexpr bool kSplit = K::kSplit;
+  constexpr int kBuffers = K::kBuffers, kLeader = 32 * K::kConverters; // kLeader: the thread that asks for pages
   extern __shared__ uint8_t raw_smem[];
   pdl_prologue();
   // the unit: 256 rows of a sequence and head; the last ones, which see most, first
   const int heads = a.cache.n_kv_heads, head = blockIdx.x % heads, unit = (int)(gridDim.x / heads) - 1 - (int)(blockIdx.x / heads);
-  auto unit0 = [&](int s) { return (int)((long)a.rows.start(s) * a.group / (kTile * kTiles)) + s; };
+  auto unit0 = [&](int s) { return (int)((long)a.rows.start(s) * a.group / K::kRowsOfBlock) + s; };
   const int s = a.rows.find(unit, unit0);
   const Rows::Span sp = a.rows.span(s);
-  const long R = (long)sp.q * a.group, row0 = (long)(unit - unit0(s)) * kTile * kTiles;
+  const long R = (long)sp.q * a.group, row0 = (long)(unit - unit0(s)) * K::kRowsOfBlock;
   if (unit < unit0(s) || R <= kMaxTokenRows || row0 >= R)
     return;
-  const int tiles = R - row0 > kTile ? 2 : 1;
+  const int tiles = (int)min((R - row0 + kTile - 1) / kTile, (long)TILES);
   auto pos_of = [&](long row) { return sp.pos + (int)(min(row, R - 1) / a.group); };
-  const Columns cols = columns(a.rows, a.window, a.n_first, pos_of(row0), pos_of(row0 + kTile * kTiles - 1));
+  const Columns cols = columns(a.rows, a.window, a.n_first, pos_of(row0), pos_of(row0 + K::kRowsOfBlock - 1));
 
   K k;
   k.base = (smem_u32(raw_smem) + 1023) & ~1023u;
@@ -210,12 +232,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
         mbar_init(smem + K::kBars + i * 8, arrivals);
     };
     init(K::kQueryFull, 1, 4 * tiles);
-    init(K::kScoreFull, 4, 1);
-    init(K::kWeightFull, 4, 4);
-    init(K::kOutDone, 2, 1);
-    init(K::kKeyFull, K::kKeyStages, 4);
+    init(K::kScoreFull, TILES * kBuffers, 1);
+    init(K::kWeightFull, TILES * kBuffers, 4);
+    init(K::kOutDone, TILES, 1);
+    init(K::kKeyFull, K::kKeyStages, 2);
     init(K::kKeyFree, K::kKeyStages, 1);
-    init(K::kValueFull, K::kValueStages, 4);
+    init(K::kValueFull, K::kValueStages, 2);
     init(K::kValueFree, K::kValueStages, 1);
     init(K::kRawFull, K::kRawStages, 1);
     init(K::kRawFree, K::kRawStages, 4);
@@ -223,7 +245,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
     *k.stop = 0;
     mbar_init_fence();
   }
-  if (warp == 12) {
+  if (warp == K::kIssuer) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(k.base + K::kTmemAt) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -231,12 +253,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
   __syncthreads();
   tc_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + K::kTmemAt);
-  auto scores_at = [&](int tile, int j) { return tmem + (tile * 2 + (j & 1)) * 64; };
-  auto out_at = [&](int tile) { return tmem + 256 + tile * D; };
+  auto scores_at = [&](int tile, int j) { return tmem + (tile * kBuffers + j % kBuffers) * 64; };
+  auto out_at = [&](int tile) { return tmem + 64 * TILES * kBuffers + tile * D; };
+  auto buffer = [&](int tile, int j) { return tile * kBuffers + j % kBuffers; };
+  auto phase = [&](int j) { return (uint32_t)(j / kBuffers & 1); };
 
-  if (warp < 8) {
+  if (warp < K::kConverters) {
     // ---- softmax: a thread per row ----------------------------------------------------
-    more_registers<152>();
+    if constexpr (TILES == 2)
+      more_registers<152>();
     const int tile = warp >> 2, r = threadIdx.x & (kTile - 1);
     const uint32_t lanes = (uint32_t)(warp & 3) << 21; // this warp's 32 lanes of tensor memory
     if (tile < tiles) {
@@ -293,26 +318,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
       // Scores of page j to weights; false: the block is to end.
       auto step = [&](auto masked, const Meta &it, int j) {
         constexpr bool kMasked = decltype(masked)::value;
-        uint32_t x[64];
+        // All 64 scores in registers where there is room (two tiles); else half by half, and the first half again for the
+        // weights, which lie where their own half's scores were.
+        constexpr int kHeld = TILES == 2 ? 64 : 32;
+        uint32_t x[kHeld];
         tmem_load32(scores_at(tile, j) + lanes, x);
-        tmem_load32(scores_at(tile, j) + lanes + 32, x + 32);
+        if constexpr (kHeld == 64)
+          tmem_load32(scores_at(tile, j) + lanes + 32, x + 32);
         tmem_loaded();
         uint32_t seen[2] = {0, 0};
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}; // four chains, so that none waits for itself
-        if constexpr (kMasked) {
-          const int hi = pos - it.token, lo = a.window > 0 ? pos - a.window - it.token : -1, first = a.n_first - it.token;
 #pragma unroll
-          for (int c = 0; c < kPage; c++) {
-            const bool sees = c <= hi && (c > lo || c < first);
-            seen[c >> 5] |= (uint32_t)sees << (c & 31);
-            tops[c & 3] = fmaxf(tops[c & 3], sees ? __uint_as_float(x[c]) : -INFINITY);
+        for (int c0 = 0; c0 < kPage; c0 += kHeld) {
+          if (c0 > 0) {
+            tmem_load32(scores_at(tile, j) + lanes + 32, x);
+            tmem_loaded();
           }
-        } else {
+          if constexpr (kMasked) {
+            const int hi = pos - it.token - c0, lo = a.window > 0 ? pos - a.window - it.token - c0 : -1, first = a.n_first - it.token - c0;
 #pragma unroll
-          for (int c = 0; c < kPage; c += 8)
+            for (int c = 0; c < kHeld; c++) {
+              const bool sees = c <= hi && (c > lo || c < first);
+              seen[(c0 + c) >> 5] |= (uint32_t)sees << (c & 31);
+              tops[c & 3] = fmaxf(tops[c & 3], sees ? __uint_as_float(x[c]) : -INFINITY);
+            }
+          } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + 4 + e])));
+            for (int c = 0; c < kHeld; c += 8)
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + 4 + e])));
+          }
         }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const float f = row_factor * it.key_scale;
@@ -340,20 +376,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
           }
         }
         const float off = (float)kTileBits - (m > -INFINITY ? m : 0.0f);
-        uint32_t w[32];
+        uint32_t w[kHeld / 2];
         float2 sums[4] = {};
 #pragma unroll
-        for (int c = 0; c < kPage; c += 2) {
-          const float2 z = fma2(make_float2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), make_float2(f, f), make_float2(off, off));
-          float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
-          if constexpr (kMasked) {
-            p.x = seen[c >> 5] >> (c & 31) & 1 ? p.x : 0.0f;
-            p.y = seen[c >> 5] >> ((c & 31) + 1) & 1 ? p.y : 0.0f;
+        for (int h0 = 0; h0 < kPage; h0 += kHeld) {
+          const int c0 = kHeld == 64 ? 0 : kHeld - h0; // the half that is still in registers first
+          if (h0 > 0) {
+            tmem_load32(scores_at(tile, j) + lanes + c0, x);
+            tmem_loaded();
           }
-          sums[c / 2 & 3] = add2(sums[c / 2 & 3], p);
-          w[c / 2] = pack_f16(p.x, p.y);
-          if constexpr (kSplit)
-            x[c / 2] = pack_rest(w[c / 2], p.x, p.y); // x[c / 2] has been read
+#pragma unroll
+          for (int c = 0; c < kHeld; c += 2) {
+            const float2 z = fma2(make_float2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), make_float2(f, f), make_float2(off, off));
+            float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+            if constexpr (kMasked) {
+              p.x = seen[(c0 + c) >> 5] >> (c & 31) & 1 ? p.x : 0.0f;
+              p.y = seen[(c0 + c) >> 5] >> ((c & 31) + 1) & 1 ? p.y : 0.0f;
+            }
+            sums[c / 2 & 3] = add2(sums[c / 2 & 3], p);
+            w[c / 2] = pack_f16(p.x, p.y);
+            if constexpr (kSplit)
+              x[c / 2] = pack_rest(w[c / 2], p.x, p.y); // x[c / 2] has been read
+          }
+          if constexpr (kHeld == 64)
+            tmem_store32(scores_at(tile, j) + lanes, w);
+          else
+            tmem_store16(scores_at(tile, j) + lanes + c0, w);
         }
         const float2 sum = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
         l += sum.x + sum.y;
@@ -364,7 +412,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
       };
       bool ok = true;
       for (;; j++) {
-        if (!(ok = k.wait_warp(K::kScoreFull + tile * 2 + (j & 1), j >> 1 & 1)))
+        if (!(ok = k.wait_warp(K::kScoreFull + buffer(tile, j), phase(j))))
           break;
         tc_after_sync();
         const Meta it = meta[j % kMeta];
@@ -377,7 +425,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
           break;
         tmem_stored();
         tc_before_sync();
-        arrive_warp(k.bar(K::kWeightFull + tile * 2 + (j & 1)));
+        arrive_warp(k.bar(K::kWeightFull + buffer(tile, j)));
       }
       if (ok && j > 0)
         ok = k.wait_warp(K::kOutDone + tile, (j - 1) & 1);
@@ -409,53 +457,58 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
         }
       }
     }
-  } else if (warp < 12) {
-    // ---- codes to fp16 ------------------------------------------------------------------
-    fewer_registers<72>();
-    const int t = threadIdx.x - 256, token = t >> 1, half = t & 1; // half of a token's codes
+  } else if (warp < K::kIssuer) {
+    // ---- codes to fp16: warps 8 and 9 the keys, 10 and 11 the values, a token per thread ----
+    if constexpr (TILES == 2)
+      fewer_registers<72>();
+    const int t = threadIdx.x & 63;
+    const bool values = warp >= K::kConverters + 2;
     const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
-    int page_of = -1, held = -32, ahead = 0, asked = 0, value_exp = 0;
+    int page_of = -1, held = -32, asked = 0, value_exp = 0;
+    unsigned there = 0; // of the columns held .. held + 31: those with a page that is still to be asked for
     float2 scale_of = make_float2(0.0f, 0.0f);
-    // Every warp goes over the table the same way; thread 0 alone asks for the bytes.  Per stage in flight:
+    // Every warp goes over the table the same way; one thread asks for the bytes.  Per raw stage:
     int ring_token[K::kRawStages];
     float2 ring_scale[K::kRawStages];
     auto ask = [&](int stage) { // the next column that has a page into `stage`; token -1: there is none
       ring_token[stage] = -1;
-      for (; ahead < cols.n; ahead = held + 32) {
-        if (ahead >= held + 32) {
-          held += 32;
-          page_of = held + lane < cols.n ? a.cache.checked(__ldg(table + cols.at(held + lane))) : -1;
-          if (page_of >= 0)
-            scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
-        }
-        const unsigned there = __ballot_sync(0xffffffffu, page_of >= 0) >> (ahead - held);
-        if (there) {
-          ahead += __ffs(there) - 1;
-          const int page = __shfl_sync(0xffffffffu, page_of, ahead - held);
-          ring_token[stage] = cols.at(ahead) * kPage;
-          ring_scale[stage].x = __shfl_sync(0xffffffffu, scale_of.x, ahead - held);
-          ring_scale[stage].y = __shfl_sync(0xffffffffu, scale_of.y, ahead - held);
-          if (t == 0) {
-            const uint32_t b = k.bar(K::kRawFull + stage);
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(K::kRawBytes) : "memory");
-            asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                             k.base + K::kRaw + stage * K::kRawBytes),
-                         "l"(a.cache.template block<D>(page, head)), "r"(K::kRawBytes), "r"(b)
-                         : "memory");
-          }
-          ahead++, asked++;
-          return;
-        }
+      while (!there && held + 32 < cols.n) {
+        held += 32;
+        page_of = held + lane < cols.n ? a.cache.checked(__ldg(table + cols.at(held + lane))) : -1;
+        if (page_of >= 0)
+          scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
+        there = __ballot_sync(0xffffffffu, page_of >= 0);
       }
+      if (!there)
+        return;
+      const int from = __ffs(there) - 1, page = __shfl_sync(0xffffffffu, page_of, from);
+      there &= there - 1;
+      ring_token[stage] = cols.at(held + from) * kPage;
+      ring_scale[stage].x = __shfl_sync(0xffffffffu, scale_of.x, from);
+      ring_scale[stage].y = __shfl_sync(0xffffffffu, scale_of.y, from);
+      if (threadIdx.x == kLeader) {
+        const uint32_t b = k.bar(K::kRawFull + stage);
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(K::kRawBytes) : "memory");
+        asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                         k.base + K::kRaw + stage * K::kRawBytes),
+                     "l"(a.cache.template block<D>(page, head)), "r"(K::kRawBytes), "r"(b)
+                     : "memory");
+      }
+      asked++;
     };
-    auto convert = [&](uint32_t from, uint32_t to, uint32_t mul, uint32_t add) { // this thread's half token
+    // The order in which a thread takes its token's pieces: such that 8 neighbouring threads' reads (rows of D
+    // bytes) and swizzled writes (rows of 128) both fall into different banks; x -> 0, 2, 3, 1 and its xor with x
+    // are both permutations.
+    const int turn_of = (0x78 >> (t & 6) & 3) | (D == 128 ? (t & 1) << 2 : 0);
+    auto convert = [&](uint32_t from, uint32_t to, uint32_t mul, uint32_t add) { // this thread's token
 #pragma unroll
-      for (int i = 0; i < D / 32; i++) { // 16 codes: two 16-byte pieces
-        const uint4 w = lds16(from + token * D + half * (D / 2) + i * 16);
+      for (int n = 0; n < D / 16; n++) { // 16 codes: two 16-byte pieces
+        const int i = n ^ turn_of;
+        const uint4 w = lds16(from + t * D + i * 16);
         const uint32_t u[4] = {biased(w.x), biased(w.y), biased(w.z), biased(w.w)};
 #pragma unroll
         for (int e = 0; e < 2; e++)
-          K::store16(to + K::swizzled(token, half * (D / 16) + i * 2 + e, kPage), scaled_pair(low_pair(u[2 * e]), mul, add),
+          K::store16(to + K::swizzled(t, i * 2 + e, kPage), scaled_pair(low_pair(u[2 * e]), mul, add),
                      scaled_pair(high_pair(u[2 * e]), mul, add), scaled_pair(low_pair(u[2 * e + 1]), mul, add),
                      scaled_pair(high_pair(u[2 * e + 1]), mul, add));
       }
@@ -465,52 +518,55 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
       ask(i);
     int used = 0;
     bool ok = true, more = true;
+    static_assert(K::kKeyStages == K::kRawStages && K::kValueStages == K::kRawStages, "one stage number for all rings");
     while (ok && more) {
 #pragma unroll
-      for (int raw = 0; raw < K::kRawStages; raw++) { // j = used, its raw stage known at compile time
+      for (int stage = 0; stage < K::kRawStages; stage++) { // of page `used`, known at compile time
         if (!ok || !more)
           break;
         const int j = used;
-        const int ks = j % K::kKeyStages, vs = j % K::kValueStages;
-        more = ring_token[raw] >= 0;
-        if (j >= K::kKeyStages && !(ok = k.wait_warp(K::kKeyFree + ks, (j / K::kKeyStages - 1) & 1)))
+        const uint32_t turn = j / K::kRawStages & 1;
+        more = ring_token[stage] >= 0;
+        if (values && !more)
           break;
-        const int v_exp = exponent_field(ring_scale[raw].y);
+        if (j >= K::kRawStages && !(ok = k.wait_warp((values ? K::kValueFree : K::kKeyFree) + stage, turn ^ 1)))
+          break;
+        const int v_exp = exponent_field(ring_scale[stage].y);
         if (more)
           value_exp = max(value_exp, v_exp);
-        if (t == 0)
-          meta[j % kMeta] = Meta{ring_token[raw], ring_scale[raw].x, value_exp, 0};
-        const uint32_t from = k.base + K::kRaw + raw * K::kRawBytes;
+        if (threadIdx.x == kLeader)
+          meta[j % kMeta] = Meta{ring_token[stage], ring_scale[stage].x, value_exp, 0};
         if (more) {
-          if (!(ok = k.wait_warp(K::kRawFull + raw, j / K::kRawStages & 1)))
+          if (!(ok = k.wait_warp(K::kRawFull + stage, turn)))
             break;
-          convert(from, k.base + K::kKeys + ks * K::kPageBytes, 0x3c003c00u, 0xe480e480u); // times 1, minus 1152
+          uint32_t mul = 0x3c003c00u, add = 0xe480e480u; // times 1, minus 1152
+          if (values)
+            value_factor(v_exp == 0 ? -99 : v_exp - value_exp + kValueBits, mul, add);
+          convert(k.base + K::kRaw + stage * K::kRawBytes + (values ? kPage * D : 0),
+                  k.base + (values ? K::kValues : K::kKeys) + stage * K::kPageBytes, mul, add);
         }
         fence_async_smem();
-        arrive_warp(k.bar(K::kKeyFull + ks));
+        arrive_warp(k.bar((values ? K::kValueFull : K::kKeyFull) + stage));
         if (!more)
           break;
-        if (j >= K::kValueStages && !(ok = k.wait_warp(K::kValueFree + vs, (j / K::kValueStages - 1) & 1)))
-          break;
-        uint32_t mul, add;
-        value_factor(v_exp == 0 ? -99 : v_exp - value_exp + kValueBits, mul, add);
-        convert(from + kPage * D, k.base + K::kValues + vs * K::kPageBytes, mul, add);
-        fence_async_smem();
-        arrive_warp(k.bar(K::kValueFull + vs));
-        arrive_warp(k.bar(K::kRawFree + raw)); // this thread has read the raw stage
+        if (lane == 0)
+          arrive(k.bar(K::kRawFree + stage)); // this warp has read its part of the raw page
         used++;
-        if (warp == 8 && !(ok = k.wait_warp(K::kRawFree + raw, j / K::kRawStages & 1)))
-          break;
-        ask(raw);
+        // the stage of the page before, which the other warps have most likely read too, gets the next page
+        const int before = (stage + K::kRawStages - 1) % K::kRawStages;
+        if (j > 0) {
+          if (warp == K::kConverters && !(ok = k.wait_warp(K::kRawFree + before, (j - 1) / K::kRawStages & 1)))
+            break;
+          ask(before);
+        }
       }
     }
-    if (t == 0 && !ok) // what is still on its way is waited for, with a limit of its own
-      for (int p = used; p < asked; p++)
+    if (threadIdx.x == kLeader && !ok) // what is still on its way is waited for, with a limit of its own
+      for (int p = used > 0 ? used - 1 : 0; p < asked; p++)
         mbar_wait_at(k.bar(K::kRawFull + p % K::kRawStages), p / K::kRawStages & 1);
   } else {
     // ---- matrix instructions --------------------------------------------------------------
     constexpr uint32_t kScoreShape = shape_of(kPage, false), kOutShape = shape_of(D, true);
-    const uint32_t leader = elected();
     const uint32_t queries = operand_low(k.base + K::kQueries, 16), keys0 = operand_low(k.base + K::kKeys, 16),
                    values0 = operand_low(k.base + K::kValues, kPage * 128);
     bool ok = k.wait_warp(K::kQueryFull, 0), more = true;
@@ -531,14 +587,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
 #pragma unroll
         for (int part = 0; part < (kSplit ? 2 : 1); part++)
 #pragma unroll
-          for (int i = 0; i < D / 16; i++)
-            mma_smem(scores_at(tile, n), q + (part * K::kQueryBytes + (i / 4) * kTile * 128 + (i % 4) * 32) / 16,
-                     keys + ((i / 4) * kPage * 128 + (i % 4) * 32) / 16, kScoreShape, part + i > 0, leader);
+          for (int i = 0; i < D / 64; i++)
+            mma4_smem(scores_at(tile, n), q + (part * K::kQueryBytes + i * kTile * 128) / 16, keys + i * (kPage * 128 / 16),
+                      kScoreShape, part + i > 0);
       }
-      tc_commit(k.bar(K::kScoreFull + tile * 2 + (n & 1)), leader); // also for the end of the pages
+      tc_commit(k.bar(K::kScoreFull + buffer(tile, n))); // also for the end of the pages
       if (tile == tiles - 1) {
         if (real) {
-          tc_commit(k.bar(K::kKeyFree + key_stage), leader);
+          tc_commit(k.bar(K::kKeyFree + key_stage));
           n++;
           if (++key_stage == K::kKeyStages)
             key_stage = 0, key_turn ^= 1;
@@ -546,12 +602,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
         more = real;
       }
     };
-    for (int i = 0; i < 2 && ok; i++)
+    for (int i = 0; i < kBuffers && ok; i++)
       for (int tile = 0; tile < tiles && ok; tile++)
         next_scores(tile);
     for (int j = 0; ok && j < n; j++) {
       for (int tile = 0; tile < tiles && ok; tile++) {
-        if (!(ok = k.wait_warp(K::kWeightFull + tile * 2 + (j & 1), j >> 1 & 1)))
+        if (!(ok = k.wait_warp(K::kWeightFull + buffer(tile, j), phase(j))))
           break;
         if (tile == 0 && !(ok = k.wait_warp(K::kValueFull + value_stage, value_turn)))
           break;
@@ -559,43 +615,52 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(Call<QT> a) {
         const uint32_t values = values0 + value_stage * (K::kPageBytes / 16);
 #pragma unroll
         for (int part = 0; part < (kSplit ? 2 : 1); part++)
-#pragma unroll
-          for (int i = 0; i < kPage / 16; i++)
-            mma_tmem(out_at(tile), scores_at(tile, j) + part * 32 + i * 8, values + i * (2048 / 16), kOutShape, j + part + i > 0,
-                     leader);
-        tc_commit(k.bar(K::kOutDone + tile), leader);
+          mma4_tmem<TILES == 2 ? 16 : 32>(out_at(tile), scores_at(tile, j) + part * 32, values, kOutShape, j + part > 0);
+        tc_commit(k.bar(K::kOutDone + tile));
         if (tile == tiles - 1)
-          tc_commit(k.bar(K::kValueFree + value_stage), leader);
+          tc_commit(k.bar(K::kValueFree + value_stage));
         next_scores(tile);
       }
       if (++value_stage == K::kValueStages)
         value_stage = 0, value_turn ^= 1;
     }
     if (!ok) { // matrix instructions still running are waited for, with a limit, before their memory is given back
-      tc_commit(k.bar(K::kDrained), leader);
+      tc_commit(k.bar(K::kDrained));
       mbar_wait_at(k.bar(K::kDrained), 0);
     }
   }
   __syncwarp();
   tc_before_sync();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == K::kIssuer) {
     tc_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
 }
 
-template <typename QT, int D> void launch_d(cudaStream_t stream, const Call<QT> &a) {
-  const long units = (long)a.rows.T * a.group / (kTile * kTiles) + a.rows.n_seqs;
-  (void)blocks_per_sm_smem(attend_tiles<QT, D>, kTileThreads, TileKernel<QT, D>::kSmem);
-  launch_kernel(attend_tiles<QT, D>, dim3((unsigned)(units * a.cache.n_kv_heads)), dim3(kTileThreads), TileKernel<QT, D>::kSmem,
-                stream, a);
+template <typename QT, int D, int TILES> void launch_with(cudaStream_t stream, const Call<QT> &a, long units) {
+  using K = TileKernel<QT, D, TILES>;
+  (void)blocks_per_sm_smem(attend_tiles<QT, D, TILES>, K::kThreads, K::kSmem);
+  launch_kernel(attend_tiles<QT, D, TILES>, dim3((unsigned)(units * a.cache.n_kv_heads)), dim3(K::kThreads), K::kSmem, stream, a);
 }
+template <typename QT> long units_of(const Call<QT> &a, int tiles) { return (long)a.rows.T * a.group / (kTile * tiles) + a.rows.n_seqs; }
 
 } // namespace
 
 template <typename QT> void launch_tiles(cudaStream_t stream, const Call<QT> &a, int head_dim) {
-  head_dim == 64 ? launch_d<QT, 64>(stream, a) : launch_d<QT, 128>(stream, a);
+  const long two = units_of(a, 2), four = units_of(a, 4);
+  if (head_dim == 128) {
+    launch_with<QT, 128, 2>(stream, a, two);
+    return;
+  }
+  // Four tiles fit tensor memory at 64 elements and bf16 rows (one part of weights); see the top for what they
+  // bring.  Where they would leave SMs without a block, two.
+  if constexpr (sizeof(QT) == 2)
+    if ((four - a.rows.n_seqs) * a.cache.n_kv_heads >= sm_count()) {
+      launch_with<QT, 64, 4>(stream, a, four);
+      return;
+    }
+  launch_with<QT, 64, 2>(stream, a, two);
 }
 template void launch_tiles<float>(cudaStream_t, const Call<float> &, int);
 template void launch_tiles<uint16_t>(cudaStream_t, const Call<uint16_t> &, int);

@@ -81,23 +81,26 @@ def attend(codes, scales, rows, n_q, row_start, kv_len, pages, max_new, scale, w
             g = h // G
             k = codes[pg, g, 0, slot].astype(np.float64) * scales[pg, g, 0].astype(np.float64)[:, None]
             v = codes[pg, g, 1, slot].astype(np.float64) * scales[pg, g, 1].astype(np.float64)[:, None]
-            for i in range(q):
-                p = pos + i
-                ok = t <= p
-                if window > 0:
-                    ok &= (t > p - window) | (t < n_first)
-                r = r0 + i
-                out[r, h] = 0
-                if not ok.any():
-                    continue
-                z = scale * (k[ok] @ x[r, h])
-                top = max(z.max(), sinks[h]) if sinks is not None else z.max()
-                w = np.exp(z - top)
-                total = w.sum() + (math.exp(sinks[h] - top) if sinks is not None else 0.0)
-                out[r, h] = w @ v[ok] / total
-                weight[r, h] = w @ np.abs(v[ok]) / total
-                reach[r, h] = (np.abs(k[ok]) @ np.abs(x[r, h])).max() * abs(scale)
-                seen[r, h], vmax[r, h] = ok.sum(), np.abs(v[ok]).max()
+            p = pos + np.arange(q)[:, None]
+            ok = t[None] <= p
+            if window > 0:
+                ok &= (t[None] > p - window) | (t[None] < n_first)
+            r = slice(r0, r0 + q)
+            z = np.where(ok, scale * (x[r, h] @ k.T), -np.inf)
+            top = z.max(1, initial=-np.inf, keepdims=True)
+            if sinks is not None:
+                top = np.maximum(top, sinks[h])
+            top = np.where(np.isfinite(top), top, 0.0)
+            w = np.exp(z - top)
+            total = w.sum(1, keepdims=True)
+            if sinks is not None:
+                total = total + np.exp(float(sinks[h]) - top)
+            any_ = ok.any(1, keepdims=True)
+            total = np.where(any_, total, 1.0)
+            out[r, h], weight[r, h] = w @ v / total, w @ np.abs(v) / total
+            reach[r, h] = np.where(ok, np.abs(x[r, h]) @ np.abs(k.T), 0).max(1, initial=0, keepdims=True) * abs(scale)
+            seen[r, h] = ok.sum(1, keepdims=True)
+            vmax[r, h] = np.where(ok, np.abs(v).max(1), 0).max(1, initial=0, keepdims=True) if len(t) else 0
     return out, weight, reach, seen, vmax
 
 

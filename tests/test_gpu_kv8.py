@@ -228,6 +228,19 @@ def test_attend_several_rows(gpu, dtype_name, n_q, heads, D, lens, new, window, 
     st.check_attend(window=window, first=first, sinks=sinks if window == 0 else None)
 
 
+@pytest.mark.parametrize("dtype_name", ["bf16", "f32"])
+@pytest.mark.parametrize("n_q,heads,D", [(64, 8, 64), (40, 8, 64), (32, 8, 128)])
+@pytest.mark.parametrize("window,first", [(0, 0), (200, 70)])
+def test_attend_prompts_that_fill_the_gpu(gpu, dtype_name, n_q, heads, D, window, first):
+    """Enough rows for a block per SM and more, a short prompt and a few single tokens among them; values of very
+    different pages, a page that is not there."""
+    pkg = gpu
+    lens, new = [1500, 1, 700, 130, 90], [1500, 1, 650, 120, 0]
+    st = Step(pkg, 65 + n_q, lens, new, n_q, heads, D, pkg.BF16 if dtype_name == "bf16" else pkg.F32, scales=(-16, 2),
+              missing=[(0, 3, -1), (2, 0, 99999)], trail=3).put()
+    st.check_attend(window=window, first=first, sinks=st.r.standard_normal(n_q).astype(np.float32))
+
+
 @pytest.mark.parametrize("in_name,out_name", [("bf16", "f32"), ("f32", "bf16")])
 @pytest.mark.parametrize("pad,offset,pad_out", [(0, 0, 0), (3, 0, 1), (8, 1, 8), (1, 3, 5)])
 def test_attend_strides_and_types(gpu, in_name, out_name, pad, offset, pad_out):
