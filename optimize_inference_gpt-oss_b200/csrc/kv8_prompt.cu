@@ -20,8 +20,6 @@
 // and their weights in two parts with two products.
 // Every wait is bounded: one that runs out is counted, tells the block's other roles, and the block frees its
 // tensor memory and ends.
-#include <type_traits>
-
 #include "kv8_attention.cuh"
 
 namespace gptoss {
@@ -51,9 +49,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// Registers a thread of this warpgroup may use from here on.  The block starts with 13 x 32 x 128; the converting warps go
-// down to 72 (128 threads) before the softmax warps' 152 (256) are granted: 9216 + 38912, and 4096 of the issuing
-// warp, are 52224 of 53248.
+// Registers a thread of this warpgroup may use from here on (the split, TileKernel, stays within what the block
+// was launched with).
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void arrive(uint32_t bar) {
@@ -126,6 +123,11 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *x) {
                GPTOSS_W8(x, 0), GPTOSS_W8(x, 8), GPTOSS_W8(x, 16), GPTOSS_W8(x, 24)
                : "memory");
 }
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t *x) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : GPTOSS_R8(x, 0), GPTOSS_R8(x, 8)
+               : "r"(at));
+}
 __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t *x) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
                GPTOSS_W8(x, 0), GPTOSS_W8(x, 8)
@@ -141,6 +143,12 @@ template <typename QT, int D, int TILES> struct TileKernel {
   static constexpr int kBuffers = TILES == 2 ? 2 : 1;                  // of scores, per tile
   static constexpr int kConverters = 4 * TILES, kIssuer = kConverters + 4, kThreads = 32 * (kIssuer + 1);
   static constexpr int kRowsOfBlock = kTile * TILES;
+  // A thread's registers: at launch (65536 over the warps rounded up to whole groups of four), and of the
+  // softmax and converting warps afterwards; the issuing warp keeps what it has.
+  static constexpr int kLaunchRegisters = TILES == 2 ? 128 : 80, kSoftmaxRegisters = TILES == 2 ? 152 : 88,
+                       kConverterRegisters = TILES == 2 ? 72 : 48;
+  static_assert(128 * TILES * kSoftmaxRegisters + 128 * kConverterRegisters + 32 * kLaunchRegisters <= kThreads * kLaunchRegisters,
+                "setmaxnreg.inc would wait for good");
   static_assert(TILES * (64 * kBuffers + D) <= 512, "tensor memory");
   static constexpr int kKeyStages = D == 64 ? 4 : kSplit ? 2 : 3, kValueStages = kKeyStages, kRawStages = D == 64 ? 4 : kSplit ? 2 : 3;
   static constexpr int kQueryBytes = kTile * D * 2;                    // of a tile and part
@@ -260,8 +268,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
 
   if (warp < K::kConverters) {
     // ---- softmax: a thread per row ----------------------------------------------------
-    if constexpr (TILES == 2)
-      more_registers<152>();
+    more_registers<K::kSoftmaxRegisters>();
     const int tile = warp >> 2, r = threadIdx.x & (kTile - 1);
     const uint32_t lanes = (uint32_t)(warp & 3) << 21; // this warp's 32 lanes of tensor memory
     if (tile < tiles) {
@@ -315,9 +322,27 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
       }
       float m = -INFINITY, l = 0.0f;
       int value_exp = 0, j = 0;
+      // What this thread's row does not see of a page gets a score below all others.  Only pages at the edge of
+      // what a tile sees come here, and the step itself has one form: with the masks in it, it ran 13 % longer
+      // over the pages that need none.
+      auto mask = [&](const Meta &it, int j) {
+        const int hi = pos - it.token, lo = a.window > 0 ? pos - a.window - it.token : -1, first = a.n_first - it.token;
+        auto ones = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }; // columns below n
+#pragma unroll 1
+        for (int c0 = 0; c0 < kPage; c0 += 32) {
+          const uint32_t sees = ones(hi + 1 - c0) & (~ones(lo + 1 - c0) | ones(first - c0));
+          uint32_t x[32];
+          tmem_load32(scores_at(tile, j) + lanes + c0, x);
+          tmem_loaded();
+#pragma unroll
+          for (int c = 0; c < 32; c++)
+            x[c] = sees & 1u << c ? x[c] : __float_as_uint(-3e38f);
+          tmem_store32(scores_at(tile, j) + lanes + c0, x);
+        }
+        tmem_stored();
+      };
       // Scores of page j to weights; false: the block is to end.
-      auto step = [&](auto masked, const Meta &it, int j) {
-        constexpr bool kMasked = decltype(masked)::value;
+      auto step = [&](const Meta &it, int j) {
         // All 64 scores in registers where there is room (two tiles); else half by half, and the first half again for the
         // weights, which lie where their own half's scores were.
         constexpr int kHeld = TILES == 2 ? 64 : 32;
@@ -326,33 +351,25 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
         if constexpr (kHeld == 64)
           tmem_load32(scores_at(tile, j) + lanes + 32, x + 32);
         tmem_loaded();
-        uint32_t seen[2] = {0, 0};
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}; // four chains, so that none waits for itself
+        float tops[4] = {-3e38f, -3e38f, -3e38f, -3e38f}; // four chains, so that none waits for itself
 #pragma unroll
         for (int c0 = 0; c0 < kPage; c0 += kHeld) {
           if (c0 > 0) {
             tmem_load32(scores_at(tile, j) + lanes + 32, x);
             tmem_loaded();
           }
-          if constexpr (kMasked) {
-            const int hi = pos - it.token - c0, lo = a.window > 0 ? pos - a.window - it.token - c0 : -1, first = a.n_first - it.token - c0;
 #pragma unroll
-            for (int c = 0; c < kHeld; c++) {
-              const bool sees = c <= hi && (c > lo || c < first);
-              seen[(c0 + c) >> 5] |= (uint32_t)sees << (c & 31);
-              tops[c & 3] = fmaxf(tops[c & 3], sees ? __uint_as_float(x[c]) : -INFINITY);
-            }
-          } else {
+          for (int c = 0; c < kHeld; c += 8)
 #pragma unroll
-            for (int c = 0; c < kHeld; c += 8)
-#pragma unroll
-              for (int e = 0; e < 4; e++)
-                tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + 4 + e])));
-          }
+            for (int e = 0; e < 4; e++)
+              tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + 4 + e])));
         }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        const float f = row_factor * it.key_scale;
-        const float now = top > -INFINITY ? fmaxf(m, top * f) : m;
+        const bool any = top > -2e38f; // real scores are below 2^28
+        // A factor that is not 0, so that what is masked stays below; 2^-100 of a score is as good as 0.
+        float f = row_factor * it.key_scale;
+        f = any ? (f < 0x1p-100f ? 0x1p-100f : f) : 1.0f;
+        const float now = any ? fmaxf(m, top * f) : m;
         if (__any_sync(0xffffffffu, now > m + kRise || it.value_exp != value_exp)) {
           const float fade = now > -INFINITY ? fast_exp2(m - now) : 1.0f;
           const float factor = fade * two_to(value_exp - it.value_exp);
@@ -364,14 +381,14 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
               return false;
             tc_after_sync();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_load32(out_at(tile) + lanes + c, o);
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_load16(out_at(tile) + lanes + c, o);
               tmem_loaded();
 #pragma unroll
-              for (int e = 0; e < 32; e++)
+              for (int e = 0; e < 16; e++)
                 o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-              tmem_store32(out_at(tile) + lanes + c, o);
+              tmem_store16(out_at(tile) + lanes + c, o);
             }
           }
         }
@@ -389,10 +406,6 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
           for (int c = 0; c < kHeld; c += 2) {
             const float2 z = fma2(make_float2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), make_float2(f, f), make_float2(off, off));
             float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
-            if constexpr (kMasked) {
-              p.x = seen[(c0 + c) >> 5] >> (c & 31) & 1 ? p.x : 0.0f;
-              p.y = seen[(c0 + c) >> 5] >> ((c & 31) + 1) & 1 ? p.y : 0.0f;
-            }
             sums[c / 2 & 3] = add2(sums[c / 2 & 3], p);
             w[c / 2] = pack_f16(p.x, p.y);
             if constexpr (kSplit)
@@ -420,8 +433,9 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
           break;
         const bool all = it.token + kPage - 1 <= min_pos &&
                          (a.window <= 0 || it.token > max_pos - a.window || it.token + kPage <= a.n_first);
-        ok = all ? step(std::false_type{}, it, j) : step(std::true_type{}, it, j);
-        if (!ok)
+        if (!all)
+          mask(it, j);
+        if (!(ok = step(it, j)))
           break;
         tmem_stored();
         tc_before_sync();
@@ -459,8 +473,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
     }
   } else if (warp < K::kIssuer) {
     // ---- codes to fp16: warps 8 and 9 the keys, 10 and 11 the values, a token per thread ----
-    if constexpr (TILES == 2)
-      fewer_registers<72>();
+    fewer_registers<K::kConverterRegisters>();
     const int t = threadIdx.x & 63;
     const bool values = warp >= K::kConverters + 2;
     const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
