@@ -670,7 +670,7 @@ template <typename QT, int D> void launch(cudaStream_t stream, const Call<QT> &a
   else
     launch_tokens<QT, D, 4>(stream, a, workspace);
   if (rows > kMaxTokenRows)
-    launch_tiles(stream, a, D);
+    launch_tiles(stream, a, D, workspace); // after the pieces above have been joined: the workspace is free again
 }
 
 template <typename QT>
@@ -697,7 +697,10 @@ extern "C" size_t gptoss_kv8_attention_workspace(const gptoss_kv8_pool_t *pool, 
   if (kv8::check_pool(pool) != GPTOSS_OK || T <= 0 || n_q_heads <= 0 || n_seqs <= 0 || max_new <= 0 ||
       n_q_heads % pool->n_kv_heads)
     return 0;
-  return kv8::Pieces::bytes(sm_count() * kv8::kMostBlocksPerSm, 32, pool->head_dim);
+  const int group = n_q_heads / pool->n_kv_heads;
+  const size_t pieces = kv8::Pieces::bytes(sm_count() * kv8::kMostBlocksPerSm, 32, pool->head_dim);
+  const bool tiles = (long)std::min(max_new, T) * group > kv8::kMaxTokenRows;
+  return std::max(pieces, tiles ? kv8::tiles_workspace(T, group, pool->n_kv_heads, n_seqs, pool->head_dim) : 0);
 }
 
 extern "C" int gptoss_kv8_attention(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int layer, int T,

@@ -80,7 +80,8 @@ template <typename QT> __device__ __forceinline__ void store4(const Call<QT> &a,
 }
 
 // Sequences of more than kMaxTokenRows rows (kv8_prompt.cu).
-template <typename QT> void launch_tiles(cudaStream_t stream, const Call<QT> &a, int head_dim);
+template <typename QT> void launch_tiles(cudaStream_t stream, const Call<QT> &a, int head_dim, void *workspace);
+size_t tiles_workspace(long T, int group, int heads, int n_seqs, int head_dim);
 
 } // namespace kv8
 } // namespace gptoss

@@ -20,6 +20,8 @@
 // and their weights in two parts with two products.
 // Every wait is bounded: one that runs out is counted, tells the block's other roles, and the block frees its
 // tensor memory and ends.
+#include <algorithm>
+
 #include "kv8_attention.cuh"
 
 namespace gptoss {
@@ -208,24 +210,60 @@ struct Meta { // of a page: its first token (-1: there are no more), key scale, 
   int value_exp, unused;
 };
 
+// The `rows` rows of a sequence and head that a block works on, and the table columns they look at.  Units are
+// numbered over the sequences: s has those from unit0(s) on.
+struct Unit {
+  Rows::Span sp;
+  int s, head;
+  long row0, R; // first row, rows of the sequence
+  Columns cols;
+  template <typename QT> __device__ __forceinline__ bool find(const Call<QT> &a, int unit, int head_, int rows) {
+    auto unit0 = [&](int i) { return (int)((long)a.rows.start(i) * a.group / rows) + i; };
+    head = head_;
+    s = a.rows.find(unit, unit0);
+    sp = a.rows.span(s);
+    R = (long)sp.q * a.group, row0 = (long)(unit - unit0(s)) * rows;
+    if (unit < unit0(s) || R <= kMaxTokenRows || row0 >= R)
+      return false;
+    cols = columns(a.rows, a.window, a.n_first, pos_of(a, row0), pos_of(a, row0 + rows - 1));
+    return true;
+  }
+  template <typename QT> __device__ __forceinline__ int pos_of(const Call<QT> &a, long row) const {
+    return sp.pos + (int)(min(row, R - 1) / a.group);
+  }
+  // Columns of one of `splits` parts.
+  __device__ __forceinline__ int column(int split, int splits) const { return (int)((long)cols.n * split / splits); }
+};
+
+// What the blocks of a unit whose columns are shared out leave for merge_parts: a row's values over its sum, and its
+// maximum and sum.
+struct Parts {
+  int splits;
+  float *o;   // [block][rows][D]
+  float2 *ml; // [block][rows]
+  static size_t bytes(long blocks, int rows, int D) { return (size_t)blocks * rows * (D * 4 + 8); }
+};
+
 template <typename QT, int D, int TILES>
-__global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT> a) {
+__global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT> a, Parts parts) {
   using K = TileKernel<QT, D, TILES>;
   constexpr bool kSplit = K::kSplit;
   constexpr int kBuffers = K::kBuffers, kLeader = 32 * K::kConverters; // kLeader: the thread that asks for pages
   extern __shared__ uint8_t raw_smem[];
   pdl_prologue();
-  // the unit: 256 rows of a sequence and head; the last ones, which see most, first
-  const int heads = a.cache.n_kv_heads, head = blockIdx.x % heads, unit = (int)(gridDim.x / heads) - 1 - (int)(blockIdx.x / heads);
-  auto unit0 = [&](int s) { return (int)((long)a.rows.start(s) * a.group / K::kRowsOfBlock) + s; };
-  const int s = a.rows.find(unit, unit0);
-  const Rows::Span sp = a.rows.span(s);
-  const long R = (long)sp.q * a.group, row0 = (long)(unit - unit0(s)) * K::kRowsOfBlock;
-  if (unit < unit0(s) || R <= kMaxTokenRows || row0 >= R)
+  // the last units of a sequence, which see most, first
+  const int heads = a.cache.n_kv_heads, split = blockIdx.x % parts.splits, index = blockIdx.x / parts.splits;
+  Unit u = {};
+  if (!u.find(a, (int)(gridDim.x / parts.splits / heads) - 1 - index / heads, index % heads, K::kRowsOfBlock))
     return;
+  const int col0 = u.column(split, parts.splits), col1 = u.column(split + 1, parts.splits);
+  if (col0 == col1)
+    return;
+  const int s = u.s, head = u.head;
+  const Rows::Span sp = u.sp;
+  const long R = u.R, row0 = u.row0;
+  const Columns cols = u.cols;
   const int tiles = (int)min((R - row0 + kTile - 1) / kTile, (long)TILES);
-  auto pos_of = [&](long row) { return sp.pos + (int)(min(row, R - 1) / a.group); };
-  const Columns cols = columns(a.rows, a.window, a.n_first, pos_of(row0), pos_of(row0 + K::kRowsOfBlock - 1));
 
   K k;
   k.base = (smem_u32(raw_smem) + 1023) & ~1023u;
@@ -276,7 +314,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
       const bool is = row < R;
       const int token = is ? (int)(row / a.group) : 0, h = head * a.group + (is ? (int)(row % a.group) : 0);
       const int pos = is ? sp.pos + token : -1;
-      const int min_pos = pos_of(row0 + tile * kTile), max_pos = pos_of(row0 + tile * kTile + kTile - 1);
+      const int min_pos = u.pos_of(a, row0 + tile * kTile), max_pos = u.pos_of(a, row0 + tile * kTile + kTile - 1);
       float row_factor;
       {
         const QT *p = a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D;
@@ -447,26 +485,34 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
         tc_after_sync();
         float f = 0.0f;
         if (l != 0.0f) { // a NaN passes
-          const float z = a.sinks ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY, top = fmaxf(m, z);
+          const bool sink = parts.splits == 1 && a.sinks;
+          const float z = sink ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY, top = fmaxf(m, z);
           const float fade = m > -INFINITY ? fast_exp2(m - top) : 1.0f;
-          const float all = l * fade + (a.sinks ? fast_exp2(z - top + (float)kTileBits) : 0.0f);
+          const float all = l * fade + (sink ? fast_exp2(z - top + (float)kTileBits) : 0.0f);
           f = fade * two_to(value_exp - 127 - kValueBits) / all;
         }
+        const size_t part = (size_t)blockIdx.x * K::kRowsOfBlock + tile * kTile + r;
+        if (parts.splits > 1 && is)
+          parts.ml[part] = make_float2(m, l * two_to(-kTileBits));
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
           if (j > 0) {
-            tmem_load32(out_at(tile) + lanes + c, o);
+            tmem_load16(out_at(tile) + lanes + c, o);
             tmem_loaded();
           }
           if (is)
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
+            for (int e = 0; e < 16; e += 4) {
               float v[4];
 #pragma unroll
               for (int i = 0; i < 4; i++)
                 v[i] = l != 0.0f ? __uint_as_float(o[e + i]) * f : 0.0f;
-              store4(a, (size_t)(sp.row + token) * a.out_row_stride + (size_t)h * D + c + e, make_float4(v[0], v[1], v[2], v[3]));
+              const float4 v4 = make_float4(v[0], v[1], v[2], v[3]);
+              if (parts.splits > 1)
+                *reinterpret_cast<float4 *>(parts.o + part * D + c + e) = v4;
+              else
+                store4(a, (size_t)(sp.row + token) * a.out_row_stride + (size_t)h * D + c + e, v4);
             }
         }
       }
@@ -477,7 +523,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
     const int t = threadIdx.x & 63;
     const bool values = warp >= K::kConverters + 2;
     const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
-    int page_of = -1, held = -32, asked = 0, value_exp = 0;
+    int page_of = -1, held = col0 - 32, asked = 0, value_exp = 0;
     unsigned there = 0; // of the columns held .. held + 31: those with a page that is still to be asked for
     float2 scale_of = make_float2(0.0f, 0.0f);
     // Every warp goes over the table the same way; one thread asks for the bytes.  Per raw stage:
@@ -485,9 +531,9 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
     float2 ring_scale[K::kRawStages];
     auto ask = [&](int stage) { // the next column that has a page into `stage`; token -1: there is none
       ring_token[stage] = -1;
-      while (!there && held + 32 < cols.n) {
+      while (!there && held + 32 < col1) {
         held += 32;
-        page_of = held + lane < cols.n ? a.cache.checked(__ldg(table + cols.at(held + lane))) : -1;
+        page_of = held + lane < col1 ? a.cache.checked(__ldg(table + cols.at(held + lane))) : -1;
         if (page_of >= 0)
           scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
         there = __ballot_sync(0xffffffffu, page_of >= 0);
@@ -651,32 +697,86 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
   }
 }
 
-template <typename QT, int D, int TILES> void launch_with(cudaStream_t stream, const Call<QT> &a, long units) {
-  using K = TileKernel<QT, D, TILES>;
-  (void)blocks_per_sm_smem(attend_tiles<QT, D, TILES>, K::kThreads, K::kSmem);
-  launch_kernel(attend_tiles<QT, D, TILES>, dim3((unsigned)(units * a.cache.n_kv_heads)), dim3(K::kThreads), K::kSmem, stream, a);
+// The parts of a unit joined, four elements per thread.
+template <typename QT, int D> __global__ void __launch_bounds__(256) merge_parts(Call<QT> a, Parts parts, int rows) {
+  constexpr int D4 = D / 4, kRowsHere = 256 / D4;
+  pdl_prologue();
+  const int heads = a.cache.n_kv_heads, index = blockIdx.x;
+  const long r = blockIdx.y * kRowsHere + threadIdx.x / D4;
+  Unit u = {};
+  if (!u.find(a, (int)(gridDim.x / heads) - 1 - index / heads, index % heads, rows) || u.row0 + r >= u.R)
+    return;
+  const int d = threadIdx.x % D4 * 4, h = u.head * a.group + (int)((u.row0 + r) % a.group);
+  const float z = a.sinks ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY;
+  auto at = [&](int split) { return ((size_t)index * parts.splits + split) * rows + r; };
+  float top = z, sum = 0.0f;
+#pragma unroll 8
+  for (int i = 0; i < parts.splits; i++)
+    if (u.column(i, parts.splits) < u.column(i + 1, parts.splits))
+      top = fmaxf(top, parts.ml[at(i)].x);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = 0; i < parts.splits; i++)
+    if (u.column(i, parts.splits) < u.column(i + 1, parts.splits)) {
+      const float2 ml = parts.ml[at(i)];
+      const float4 x = *reinterpret_cast<const float4 *>(parts.o + at(i) * D + d);
+      const float part = ml.y != 0.0f ? ml.y * fast_exp2(ml.x - top) : 0.0f; // a NaN passes
+      sum += part;
+      acc.x += part * x.x, acc.y += part * x.y, acc.z += part * x.z, acc.w += part * x.w;
+    }
+  if (sum != 0.0f && a.sinks)
+    sum += fast_exp2(z - top);
+  const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
+  store4(a, (size_t)(u.sp.row + (u.row0 + r) / a.group) * a.out_row_stride + (size_t)h * D + d,
+         make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
 }
-template <typename QT> long units_of(const Call<QT> &a, int tiles) { return (long)a.rows.T * a.group / (kTile * tiles) + a.rows.n_seqs; }
+
+long units_of(long T, int group, int n_seqs, int tiles) { return T * group / (kTile * tiles) + n_seqs; }
+// Parts that a unit's columns are cut into where there are few units: about two blocks per SM, counting the units
+// that the call's sizes allow for (the true number may be half).
+int splits_for(long blocks) { return (int)std::min(32l, std::max(1l, 2l * sm_count() / std::max(blocks, 1l))); }
+
+template <typename QT, int D, int TILES>
+void launch_with(cudaStream_t stream, const Call<QT> &a, long units, int splits, void *workspace) {
+  using K = TileKernel<QT, D, TILES>;
+  const long blocks = units * a.cache.n_kv_heads;
+  Parts parts = {splits, static_cast<float *>(workspace), nullptr};
+  parts.ml = reinterpret_cast<float2 *>(parts.o + (size_t)blocks * splits * K::kRowsOfBlock * D);
+  (void)blocks_per_sm_smem(attend_tiles<QT, D, TILES>, K::kThreads, K::kSmem);
+  launch_kernel(attend_tiles<QT, D, TILES>, dim3((unsigned)(blocks * splits)), dim3(K::kThreads), K::kSmem, stream, a, parts);
+  if (splits > 1) {
+    const PdlScope chained(GPTOSS_PDL);
+    launch_kernel(merge_parts<QT, D>, dim3((unsigned)blocks, K::kRowsOfBlock / (1024 / D)), dim3(256), 0, stream, a, parts,
+                  (int)K::kRowsOfBlock);
+  }
+}
 
 } // namespace
 
-template <typename QT> void launch_tiles(cudaStream_t stream, const Call<QT> &a, int head_dim) {
-  const long two = units_of(a, 2), four = units_of(a, 4);
+size_t tiles_workspace(long T, int group, int heads, int n_seqs, int head_dim) {
+  const long blocks = units_of(T, group, n_seqs, 2) * heads;
+  const int splits = splits_for(blocks);
+  return splits > 1 ? Parts::bytes(blocks * splits, 2 * kTile, head_dim) : 0;
+}
+
+template <typename QT> void launch_tiles(cudaStream_t stream, const Call<QT> &a, int head_dim, void *workspace) {
+  const long two = units_of(a.rows.T, a.group, a.rows.n_seqs, 2), four = units_of(a.rows.T, a.group, a.rows.n_seqs, 4);
+  const int splits = std::min(splits_for(two * a.cache.n_kv_heads), std::max(1, a.rows.pages_stride / 4));
   if (head_dim == 128) {
-    launch_with<QT, 128, 2>(stream, a, two);
+    launch_with<QT, 128, 2>(stream, a, two, splits, workspace);
     return;
   }
   // Four tiles fit tensor memory at 64 elements and bf16 rows (one part of weights); see the top for what they
   // bring.  Where they would leave SMs without a block, two.
   if constexpr (sizeof(QT) == 2)
     if ((four - a.rows.n_seqs) * a.cache.n_kv_heads >= sm_count()) {
-      launch_with<QT, 64, 4>(stream, a, four);
+      launch_with<QT, 64, 4>(stream, a, four, 1, workspace);
       return;
     }
-  launch_with<QT, 64, 2>(stream, a, two);
+  launch_with<QT, 64, 2>(stream, a, two, splits, workspace);
 }
-template void launch_tiles<float>(cudaStream_t, const Call<float> &, int);
-template void launch_tiles<uint16_t>(cudaStream_t, const Call<uint16_t> &, int);
+template void launch_tiles<float>(cudaStream_t, const Call<float> &, int, void *);
+template void launch_tiles<uint16_t>(cudaStream_t, const Call<uint16_t> &, int, void *);
 
 } // namespace kv8
 } // namespace gptoss

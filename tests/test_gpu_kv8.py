@@ -308,6 +308,19 @@ def test_attend_long_context_few_rows(gpu, dtype_name):
     st.check_attend(window=5000, first=100)
 
 
+@pytest.mark.parametrize("dtype_name", ["bf16", "f32"])
+@pytest.mark.parametrize("n_q,heads,D,lens,new", [(16, 2, 64, [5000, 300, 3], [20, 12, 1]), (16, 1, 128, [4099], [5]),
+                                                  (64, 8, 64, [3000], [33]), (12, 3, 128, [2500, 130], [40, 100])])
+def test_attend_long_context_some_rows(gpu, dtype_name, n_q, heads, D, lens, new):
+    """More rows than the token kernel takes, too few for a block per SM: the context is shared out and joined; with
+    parts that see nothing, a page that is not there, a row with a NaN."""
+    pkg = gpu
+    st = Step(pkg, 97, lens, new, n_q, heads, D, pkg.BF16 if dtype_name == "bf16" else pkg.F32, missing=[(0, 1, -1), (0, 17, -1)]).put()
+    st.check_attend(sinks=st.r.standard_normal(n_q).astype(np.float32))
+    st.check_attend(window=1000, first=70)
+    st.check_attend(window=64, first=0)
+
+
 def test_attend_masked_query_does_not_leak(gpu):
     """NaN and infinities in one row's query show in that row alone."""
     pkg = gpu
