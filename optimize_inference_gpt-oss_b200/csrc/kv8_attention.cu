@@ -57,7 +57,7 @@ __device__ __forceinline__ int token_of(int n) { return n ^ ((n >> 1) & 1); }
 
 // Scores and outputs are kept transposed (tokens x rows, elements x rows): the 8-wide side of the
 // matrix instruction is the rows', so that 8 rows (a group of 8 query heads and one token) waste nothing.
-template <typename QT, int D, int RB> struct TokenKernel {
+template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
   static constexpr bool kSplit = sizeof(QT) == 4;                     // two fp16 parts
   static constexpr int CH = (D == 64 ? 64 : 32) / (RB == 4 ? 2 : 1);  // tokens of a step
   static constexpr int kSteps = kPage / CH;                           // steps of a page
@@ -65,9 +65,11 @@ template <typename QT, int D, int RB> struct TokenKernel {
   static constexpr int kRows = 8 * RB;
   static constexpr int kPitch = D + 4; // floats of a row in shared memory
   static constexpr int kPart = CH * D;              // bytes of a step's keys, and of its values
-  static constexpr int kDepth = 8192 / kPart;       // steps' keys (and values) in a warp's ring
+  // Steps' keys (and values) in a warp's ring.  Short items have hardly more than one step per warp: half the
+  // ring, and four blocks on an SM instead of three.
+  static constexpr int kDepth = (WHOLE ? 4096 : 8192) / kPart;
   static constexpr int kResult = kRows * (kPitch * 4 + 8); // a warp's results, which lie where its ring was
-  static constexpr int kRing = 2 * kDepth * kPart > kResult ? 2 * kDepth * kPart : kResult; // 16 KB per warp
+  static constexpr int kRing = 2 * kDepth * kPart > kResult ? 2 * kDepth * kPart : kResult; // 8 or 16 KB per warp
   static constexpr int kSmem = kTokenWarps * (kRing + 2 * kDepth * 8 + kDepth * 16);
   using VWord = typename std::conditional<D == 64, uint2, uint4>::type;
 
@@ -317,7 +319,7 @@ template <typename QT, int D, int RB> struct TokenKernel {
     int page_of = -1, held = -32, ahead = 0; // lane l has the page and scales of step held + l; steps before `ahead` are asked for
     float2 scale_of = make_float2(0.0f, 0.0f);
     int asked = done; // parts
-    auto ask_keys = [&]() { // of the next step that has a page
+    auto ask_keys = [&](bool values_too) { // of the next step that has a page
       for (; ahead < steps; ahead = held + 32) {
         if (ahead >= held + 32) {
           held += 32;
@@ -330,11 +332,16 @@ template <typename QT, int D, int RB> struct TokenKernel {
         if (there) {
           ahead += __ffs(there) - 1;
           const int page = __shfl_sync(0xffffffffu, page_of, ahead - held);
-          const float ks = __shfl_sync(0xffffffffu, scale_of.x, ahead - held), vs = __shfl_sync(0xffffffffu, scale_of.y, ahead - held);
-          if (lane == 0) {
-            slots[asked % kDepth] = make_int4(page, j0 + kTokenWarps * ahead, __float_as_int(ks), __float_as_int(vs));
-            start(asked, 0, a.cache.template block<D>(page, head), (j0 + kTokenWarps * ahead) % kSteps);
+          const int step = j0 + kTokenWarps * ahead;
+          const int8_t *block = a.cache.template block<D>(page, head);
+          if (lane == 0) { // the copies first: they need the page alone, and its scales may still be on their way
+            start(asked, 0, block, step % kSteps);
+            if (values_too)
+              start(asked, 1, block, step % kSteps);
           }
+          const float ks = __shfl_sync(0xffffffffu, scale_of.x, ahead - held), vs = __shfl_sync(0xffffffffu, scale_of.y, ahead - held);
+          if (lane == 0)
+            slots[asked % kDepth] = make_int4(page, step, __float_as_int(ks), __float_as_int(vs));
           asked++, ahead++;
           return;
         }
@@ -348,10 +355,8 @@ template <typename QT, int D, int RB> struct TokenKernel {
     };
     begin();
 #pragma unroll 1
-    for (int d = 0; d < kDepth; d++) {
-      ask_keys();
-      ask_values(done + d);
-    }
+    for (int d = 0; d < kDepth; d++)
+      ask_keys(true);
     load_queries(a, sp, head, row0); // while the first parts are on their way
 #pragma unroll 1
     for (; done < asked; done++) {
@@ -364,7 +369,7 @@ template <typename QT, int D, int RB> struct TokenKernel {
       float w[RB][TT][4];
       scores(w, part_at(done, 0));
       __syncwarp(); // every lane has read the keys and the slot
-      ask_keys();
+      ask_keys(false);
       const int token = cols.at(it.y / kSteps) * kPage + (it.y % kSteps) * CH, v_exp = exponent_field(__int_as_float(it.w));
       if (token + CH - 1 <= min_pos && (a.window <= 0 || token > max_pos - a.window || token + CH <= a.n_first))
         weigh<false>(w, __int_as_float(it.z), v_exp, token, a.window, a.n_first);
@@ -468,9 +473,9 @@ __device__ __forceinline__ GroupRange group_range(const Rows::Span &sp, int grou
 // WHOLE: a block per (sequence, head, row group), for calls whose items are all short.  Otherwise all
 // items' columns, in order, in equal pieces.
 template <typename QT, int D, int RB, bool WHOLE>
-__global__ void __launch_bounds__(kTokenWarps * 32, RB <= 2 ? 3 : 2)
+__global__ void __launch_bounds__(kTokenWarps * 32, RB <= 2 ? (WHOLE && D == 64 && RB == 1 ? 4 : 3) : 2)
     attend_tokens(Call<QT> a, int groups, Pieces pieces) {
-  using K = TokenKernel<QT, D, RB>;
+  using K = TokenKernel<QT, D, RB, WHOLE>;
   pdl_prologue();
   K k;
   k.setup();
@@ -634,12 +639,12 @@ constexpr int kMostBlocksPerSm = 4;
 
 // Blocks of attend_tokens on the current device; the workspace is laid out for this many.
 template <typename QT, int D, int RB> int token_grid() {
-  const int per_sm = blocks_per_sm_smem(attend_tokens<QT, D, RB, false>, kTokenWarps * 32, TokenKernel<QT, D, RB>::kSmem);
+  const int per_sm = blocks_per_sm_smem(attend_tokens<QT, D, RB, false>, kTokenWarps * 32, TokenKernel<QT, D, RB, false>::kSmem);
   return sm_count() * std::min(std::max(per_sm, 1), kMostBlocksPerSm);
 }
 template <typename QT, int D, int RB>
 void launch_tokens(cudaStream_t stream, const Call<QT> &a, void *workspace) {
-  using K = TokenKernel<QT, D, RB>;
+  using K = TokenKernel<QT, D, RB, false>;
   const int heads = a.cache.n_kv_heads;
   const long most_rows = std::min((long)a.rows.max_new * a.group, (long)kMaxTokenRows);
   const int groups = (int)((most_rows + K::kRows - 1) / K::kRows);
@@ -650,8 +655,9 @@ void launch_tokens(cudaStream_t stream, const Call<QT> &a, void *workspace) {
                              (long)a.rows.pages_stride);
   const dim3 block(kTokenWarps * 32);
   if (most <= 2 * kMinPages && items <= 0x7fffffff) {
-    (void)blocks_per_sm_smem(attend_tokens<QT, D, RB, true>, kTokenWarps * 32, K::kSmem);
-    launch_kernel(attend_tokens<QT, D, RB, true>, dim3((unsigned)items), block, K::kSmem, stream, a, groups, Pieces{});
+    constexpr int kSmem = TokenKernel<QT, D, RB, true>::kSmem;
+    (void)blocks_per_sm_smem(attend_tokens<QT, D, RB, true>, kTokenWarps * 32, kSmem);
+    launch_kernel(attend_tokens<QT, D, RB, true>, dim3((unsigned)items), block, kSmem, stream, a, groups, Pieces{});
     return;
   }
   const int grid = (int)std::min((long)token_grid<QT, D, RB>(), items * most);

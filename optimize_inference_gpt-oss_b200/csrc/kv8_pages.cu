@@ -6,12 +6,14 @@
 // from a list that the first one left in the workspace.  Nothing comes back to the host.
 //
 // Copies: 16 KB pieces of (pair, layer), 256 threads with four 16-byte loads each in flight and
-// eight blocks per SM (128 KB in flight per SM), which is what a plain copy needs to run at the
-// memory's speed.
+// six blocks per SM (96 KB in flight per SM), which is what a plain copy needs to run at the
+// memory's speed; the same launch first brings the tables in line with the plan.
 // Decisions: bound by latency.  The reference counts are looked through 8192 at a time, eight
 // independent coalesced loads per thread, ranks from warp ballots; a search for free pages stops as
 // soon as it has enough.
 #include <limits.h>
+
+#include <algorithm>
 
 #include "kv8.cuh"
 
@@ -288,32 +290,36 @@ __global__ void __launch_bounds__(kThreads)
     *ws.count = found;
 }
 
-// The children's rows, then (copy_pairs) their last pages: a warp per fork.
-__global__ void __launch_bounds__(256)
-    write_forks(Table t, int n, const int *__restrict__ parents, const int *__restrict__ children, Scratch ws) {
-  pdl_prologue();
-  const int lane = threadIdx.x & 31;
-  for (int i = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < n; i += (gridDim.x * blockDim.x) >> 5) {
-    if (ws.a[i] == 0)
-      continue;
-    const int p = parents[i], c = children[i], len = t.kv_len[p], full = len / kPage;
-    for (int j = lane; j < full; j += 32) {
-      const int page = t.row(p)[j];
-      if (t.is_page(page)) {
-        t.row(c)[j] = page;
-        atomicAdd(t.refs + page, 1);
+// The children's rows, a warp per fork.
+struct WriteForks {
+  Table t;
+  int n;
+  const int *parents, *children;
+  Scratch ws;
+  __device__ __forceinline__ void operator()() const {
+    const int lane = threadIdx.x & 31;
+    for (int i = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < n; i += (gridDim.x * blockDim.x) >> 5) {
+      if (ws.a[i] == 0)
+        continue;
+      const int p = parents[i], c = children[i], len = t.kv_len[p], full = len / kPage;
+      for (int j = lane; j < full; j += 32) {
+        const int page = t.row(p)[j];
+        if (t.is_page(page)) {
+          t.row(c)[j] = page;
+          atomicAdd(t.refs + page, 1);
+        }
       }
-    }
-    if (lane == 0) {
-      t.kv_len[c] = len;
-      if (ws.a[i] == 2) {
-        const int page = ws.dst[ws.b[i]];
-        t.row(c)[full] = page;
-        t.refs[page] = 1;
+      if (lane == 0) {
+        t.kv_len[c] = len;
+        if (ws.a[i] == 2) {
+          const int page = ws.dst[ws.b[i]];
+          t.row(c)[full] = page;
+          t.refs[page] = 1;
+        }
       }
     }
   }
-}
+};
 
 // ---- compact --------------------------------------------------------------------------
 
@@ -337,15 +343,21 @@ __global__ void __launch_bounds__(kThreads) plan_compaction(Table t, int *remap,
     *n_live_out = n_live, *ws.count = holes;
 }
 
-__global__ void __launch_bounds__(256) renumber_tables(Table t, const int *__restrict__ remap) {
-  pdl_prologue();
-  const long all = (long)t.n_seqs * t.stride;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long)gridDim.x * blockDim.x) {
-    const int page = t.pages[i];
-    if (t.is_page(page))
-      t.pages[i] = remap[page];
+struct RenumberTables {
+  Table t;
+  const int *remap;
+  __device__ __forceinline__ void operator()() const {
+    const long all = (long)t.n_seqs * t.stride;
+    for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long)gridDim.x * blockDim.x) {
+      const int page = t.pages[i];
+      if (t.is_page(page))
+        t.pages[i] = remap[page];
+    }
   }
-}
+};
+struct Nothing {
+  __device__ __forceinline__ void operator()() const {}
+};
 
 // ---- the pages' bytes -------------------------------------------------------------------
 
@@ -358,10 +370,13 @@ struct Pool {
   int page_scales, n_layers, n_pages;
 };
 
-// Pairs (src[i], dst[i]), i < *count (or n where count is NULL), in every layer.
-__global__ void __launch_bounds__(256, 8)
-    copy_pairs(Pool pool, int n, const int *count, const int *__restrict__ src, const int *__restrict__ dst) {
+// What a plan changes in the tables (`first`), then pairs (src[i], dst[i]), i < *count (or n where count is NULL),
+// in every layer.  The two do not meet: the pairs come from the plan's list alone.
+template <typename First>
+__global__ void __launch_bounds__(256, 6)
+    copy_pairs(First first, Pool pool, int n, const int *count, const int *__restrict__ src, const int *__restrict__ dst) {
   pdl_prologue();
+  first();
   if (count)
     n = *count;
   const long pieces = (pool.page_bytes + kPiece - 1) / kPiece, all = (long)n * pool.n_layers * pieces;
@@ -390,14 +405,15 @@ __global__ void __launch_bounds__(256, 8)
   }
 }
 
-void launch_copies(cudaStream_t stream, const gptoss_kv8_pool_t *p, int n_most, const int *count, const int *src,
-                   const int *dst) {
+// first_blocks: blocks that `first` has work for.
+template <typename First>
+void launch_copies(cudaStream_t stream, First first, long first_blocks, const gptoss_kv8_pool_t *p, int n_most, const int *count,
+                   const int *src, const int *dst) {
   const Pool pool = {p->codes, p->scales, (long)p->n_kv_heads * 2 * kPage * p->head_dim, p->n_kv_heads * 2, p->n_layers,
                      p->n_pages};
   const long all = (long)n_most * p->n_layers * ((pool.page_bytes + kPiece - 1) / kPiece);
-  if (all == 0)
-    return;
-  launch_kernel(copy_pairs, dim3(row_grid(all, 8)), dim3(256), 0, stream, pool, n_most, count, src, dst);
+  launch_kernel(copy_pairs<First>, dim3(row_grid(std::max(all, first_blocks), 6)), dim3(256), 0, stream, first, pool, n_most, count,
+                src, dst);
 }
 
 int check_table(int n_seqs, const int *pages, int pages_stride, int n_pages, const int *refs) {
@@ -500,8 +516,7 @@ extern "C" int gptoss_kv8_fork(gptoss_stream_t stream, const gptoss_kv8_pool_t *
   const kv8::Scratch ws = kv8::Scratch::at(workspace, pool->n_pages, n_seqs);
   launch_kernel(kv8::plan_forks, dim3(1), dim3(kv8::kThreads), 0, as_stream(stream), t, n, parents, children, served, ws);
   const kv8::Chained chained;
-  launch_kernel(kv8::write_forks, dim3(row_grid((n + 7) / 8, 8)), dim3(256), 0, as_stream(stream), t, n, parents, children, ws);
-  kv8::launch_copies(as_stream(stream), pool, n, ws.count, ws.src, ws.dst);
+  kv8::launch_copies(as_stream(stream), kv8::WriteForks{t, n, parents, children, ws}, (n + 7) / 8, pool, n, ws.count, ws.src, ws.dst);
   return launch_status();
 }
 
@@ -526,10 +541,9 @@ extern "C" int gptoss_kv8_compact(gptoss_stream_t stream, const gptoss_kv8_pool_
   const kv8::Scratch ws = kv8::Scratch::at(workspace, pool->n_pages, n_seqs);
   launch_kernel(kv8::plan_compaction, dim3(1), dim3(kv8::kThreads), 0, as_stream(stream), t, remap, n_live_out, ws);
   const kv8::Chained chained;
-  launch_kernel(kv8::renumber_tables, dim3(row_grid(((long)n_seqs * pages_stride + 255) / 256, 8)), dim3(256), 0,
-                as_stream(stream), t, remap);
   // at most half of the pages can move: as many as there are holes below, and live pages above
-  kv8::launch_copies(as_stream(stream), pool, pool->n_pages / 2, ws.count, ws.src, ws.dst);
+  kv8::launch_copies(as_stream(stream), kv8::RenumberTables{t, remap}, ((long)n_seqs * pages_stride + 255) / 256, pool,
+                     pool->n_pages / 2, ws.count, ws.src, ws.dst);
   return launch_status();
 }
 
@@ -549,6 +563,6 @@ extern "C" int gptoss_kv8_copy_pages(gptoss_stream_t stream, const gptoss_kv8_po
   GPTOSS_SPAN(dst, (size_t)n * 4);
   GPTOSS_SPAN(pool->codes, kv8::layer_codes(pool) * pool->n_layers);
   GPTOSS_SPAN(pool->scales, kv8::layer_scales(pool) * pool->n_layers * 4);
-  kv8::launch_copies(as_stream(stream), pool, n, nullptr, src, dst);
+  kv8::launch_copies(as_stream(stream), kv8::Nothing{}, 0, pool, n, nullptr, src, dst);
   return launch_status();
 }
