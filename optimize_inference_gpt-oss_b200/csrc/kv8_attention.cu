@@ -474,7 +474,7 @@ __device__ __forceinline__ GroupRange group_range(const Rows::Span &sp, int grou
 // items' columns, in order, in equal pieces.
 template <typename QT, int D, int RB, bool WHOLE>
 __global__ void __launch_bounds__(kTokenWarps * 32, RB <= 2 ? (WHOLE && D == 64 && RB == 1 ? 4 : 3) : 2)
-    attend_tokens(Call<QT> a, int groups, Pieces pieces) {
+    attend_tokens(Call<QT> a, int above, int upto, int groups, Pieces pieces) { // sequences of above < rows <= upto
   using K = TokenKernel<QT, D, RB, WHOLE>;
   pdl_prologue();
   K k;
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32, RB <= 2 ? (WHOLE && D == 64 
   const int heads = a.cache.n_kv_heads;
   auto n_groups = [&](const Rows::Span &sp) {
     const long R = (long)sp.q * a.group;
-    return R > kMaxTokenRows ? 0 : (int)(R + K::kRows - 1) / K::kRows;
+    return R > upto || R <= above ? 0 : (int)(R + K::kRows - 1) / K::kRows;
   };
   if constexpr (WHOLE) {
     const int rg = blockIdx.x % groups, rest = blockIdx.x / groups, head = rest % heads, s = rest / heads;
@@ -643,10 +643,10 @@ template <typename QT, int D, int RB> int token_grid() {
   return sm_count() * std::min(std::max(per_sm, 1), kMostBlocksPerSm);
 }
 template <typename QT, int D, int RB>
-void launch_tokens(cudaStream_t stream, const Call<QT> &a, void *workspace) {
+void launch_tokens(cudaStream_t stream, const Call<QT> &a, int above, int upto, void *workspace) {
   using K = TokenKernel<QT, D, RB, false>;
   const int heads = a.cache.n_kv_heads;
-  const long most_rows = std::min((long)a.rows.max_new * a.group, (long)kMaxTokenRows);
+  const long most_rows = std::min((long)a.rows.max_new * a.group, (long)upto);
   const int groups = (int)((most_rows + K::kRows - 1) / K::kRows);
   const long items = (long)a.rows.n_seqs * heads * groups;
   // columns of an item at most: the window and what its rows span, the first tokens, the table
@@ -657,26 +657,34 @@ void launch_tokens(cudaStream_t stream, const Call<QT> &a, void *workspace) {
   if (most <= 2 * kMinPages && items <= 0x7fffffff) {
     constexpr int kSmem = TokenKernel<QT, D, RB, true>::kSmem;
     (void)blocks_per_sm_smem(attend_tokens<QT, D, RB, true>, kTokenWarps * 32, kSmem);
-    launch_kernel(attend_tokens<QT, D, RB, true>, dim3((unsigned)items), block, kSmem, stream, a, groups, Pieces{});
+    launch_kernel(attend_tokens<QT, D, RB, true>, dim3((unsigned)items), block, kSmem, stream, a, above, upto, groups, Pieces{});
     return;
   }
   const int grid = (int)std::min((long)token_grid<QT, D, RB>(), items * most);
   const Pieces pieces = Pieces::at(workspace, grid, K::kRows, D);
-  launch_kernel(attend_tokens<QT, D, RB, false>, dim3(grid), block, K::kSmem, stream, a, groups, pieces);
+  launch_kernel(attend_tokens<QT, D, RB, false>, dim3(grid), block, K::kSmem, stream, a, above, upto, groups, pieces);
   const PdlScope chained(GPTOSS_PDL);
   launch_kernel(merge_pieces<QT, D, RB>, dim3(grid, RB), dim3(kMergeThreads), 0, stream, a, pieces);
 }
 
+// One launch after the other on the same workspace: each has joined its pieces before the next begins.
 template <typename QT, int D> void launch(cudaStream_t stream, const Call<QT> &a, void *workspace) {
   const long rows = (long)a.rows.max_new * a.group;
   if (rows <= 8)
-    launch_tokens<QT, D, 1>(stream, a, workspace);
+    launch_tokens<QT, D, 1>(stream, a, 0, 8, workspace);
   else if (rows <= 16)
-    launch_tokens<QT, D, 2>(stream, a, workspace);
-  else
-    launch_tokens<QT, D, 4>(stream, a, workspace);
+    launch_tokens<QT, D, 2>(stream, a, 0, 16, workspace);
+  else {
+    // Sequences may be of very different row counts: single tokens among chunks of prompts.  Those get the kernel for
+    // 8 rows (64 sequences over 0.57 GB, one with 512 rows and the others with one: 294 us instead of 435; a batch that has
+    // none such pays 4 us for asking), unless the sizes say that all have the same.
+    const bool mixed = a.group <= 8 && (long)a.rows.n_seqs * a.rows.max_new > a.rows.T;
+    if (mixed)
+      launch_tokens<QT, D, 1>(stream, a, 0, 8, workspace);
+    launch_tokens<QT, D, 4>(stream, a, mixed ? 8 : 0, kMaxTokenRows, workspace);
+  }
   if (rows > kMaxTokenRows)
-    launch_tiles(stream, a, D, workspace); // after the pieces above have been joined: the workspace is free again
+    launch_tiles(stream, a, D, workspace);
 }
 
 template <typename QT>
