@@ -315,45 +315,64 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
       const int token = is ? (int)(row / a.group) : 0, h = head * a.group + (is ? (int)(row % a.group) : 0);
       const int pos = is ? sp.pos + token : -1;
       const int min_pos = u.pos_of(a, row0 + tile * kTile), max_pos = u.pos_of(a, row0 + tile * kTile + kTile - 1);
-      float row_factor;
+      // The warp's 32 queries, D / 8 lanes to a row and 8 elements to a lane, so that loads are of whole lines (a
+      // thread per row took 6 us for them); then each lane keeps the factor of its own row.
+      float row_factor = 0.0f;
       {
-        const QT *p = a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D;
-        float top = 0.0f;
-        bool odd = false;
-#pragma unroll 16
-        for (int c = 0; c < D; c += 4) {
-          float v[4];
-          load4(p + c, a.q_vec, v);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            odd = odd || !(fabsf(v[e]) <= 3.402823466e38f);
-            top = fmaxf(top, fabsf(v[e]));
-          }
-        }
-        // largest |q| into [2^13, 2^14), as in kv8_attention.cu
-        const int up = odd || top == 0.0f ? 0 : max(min(13 - (exponent_field(top) - 127), 126), -126);
-        const float f = two_to(up) * (a.scale < 0.0f ? -1.0f : 1.0f);
-        row_factor = odd ? NAN : fabsf(a.scale) * kLog2e * two_to(-up);
+        constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes, kAhead = 4;
+        const int piece = lane % kLanes, sub = lane / kLanes;
         const uint32_t to = k.base + K::kQueries + tile * (kSplit ? 2 : 1) * K::kQueryBytes;
-#pragma unroll 2
-        for (int c = 0; c < D / 8; c++) {
-          uint32_t w[4], rest[4];
+        const long first = row0 + tile * kTile + (warp & 3) * 32;
+#pragma unroll 1
+        for (int i0 = 0; i0 < kLanes; i0 += kAhead) {
+          float v[kAhead][8];
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            float v[4];
-            load4(p + 8 * c + 4 * half, a.q_vec, v);
+          for (int n = 0; n < kAhead; n++) {
+            const long at = min(first + (i0 + n) * kRowsAtOnce + sub, R - 1);
+            const QT *p = a.qkv + (size_t)(sp.row + (int)(at / a.group)) * a.row_stride +
+                          (size_t)(head * a.group + (int)(at % a.group)) * D + piece * 8;
+            float lo[4], hi[4];
+            load4(p, a.q_vec, lo);
+            load4(p + 4, a.q_vec, hi);
 #pragma unroll
             for (int e = 0; e < 4; e++)
-              v[e] = odd || !is ? 0.0f : v[e] * f;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              w[2 * half + e] = pack_f16(v[2 * e], v[2 * e + 1]);
-              rest[2 * half + e] = pack_rest(w[2 * half + e], v[2 * e], v[2 * e + 1]);
-            }
+              v[n][e] = lo[e], v[n][4 + e] = hi[e];
           }
-          K::store16(to + K::swizzled(r, c, kTile), w[0], w[1], w[2], w[3]);
-          if constexpr (kSplit)
-            K::store16(to + K::kQueryBytes + K::swizzled(r, c, kTile), rest[0], rest[1], rest[2], rest[3]);
+#pragma unroll
+          for (int n = 0; n < kAhead; n++) {
+            const int i = i0 + n, row_here = i * kRowsAtOnce + sub; // of the warp's 32
+            float top = 0.0f;
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              odd = odd || !(fabsf(v[n][e]) <= 3.402823466e38f);
+              top = fmaxf(top, fabsf(v[n][e]));
+            }
+#pragma unroll
+            for (int x = 1; x < kLanes; x <<= 1) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              odd = __shfl_xor_sync(0xffffffffu, (int)odd, x) || odd;
+            }
+            const bool real = first + row_here < R;
+            // largest |q| into [2^13, 2^14), as in kv8_attention.cu
+            const int up = odd || !real || top == 0.0f ? 0 : max(min(13 - (exponent_field(top) - 127), 126), -126);
+            const float f = two_to(up) * (a.scale < 0.0f ? -1.0f : 1.0f);
+            const float factor = odd && real ? NAN : fabsf(a.scale) * kLog2e * two_to(-up);
+            uint32_t w[4], rest[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float x = odd || !real ? 0.0f : v[n][2 * e] * f, y = odd || !real ? 0.0f : v[n][2 * e + 1] * f;
+              w[e] = pack_f16(x, y);
+              rest[e] = pack_rest(w[e], x, y);
+            }
+            const int r_here = (warp & 3) * 32 + row_here;
+            K::store16(to + K::swizzled(r_here, piece, kTile), w[0], w[1], w[2], w[3]);
+            if constexpr (kSplit)
+              K::store16(to + K::kQueryBytes + K::swizzled(r_here, piece, kTile), rest[0], rest[1], rest[2], rest[3]);
+            const float mine = __shfl_sync(0xffffffffu, factor, lane % kRowsAtOnce * kLanes);
+            if (lane / kRowsAtOnce == i)
+              row_factor = mine;
+          }
         }
         fence_async_smem();
         arrive_warp(k.bar(K::kQueryFull));
@@ -491,29 +510,47 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
           const float all = l * fade + (sink ? fast_exp2(z - top + (float)kTileBits) : 0.0f);
           f = fade * two_to(value_exp - 127 - kValueBits) / all;
         }
+        const bool apart = parts.splits > 1;
         const size_t part = (size_t)blockIdx.x * K::kRowsOfBlock + tile * kTile + r;
-        if (parts.splits > 1 && is)
+        if (apart && is)
           parts.ml[part] = make_float2(m, l * two_to(-kTileBits));
+        // Where the row goes; then 32 elements at a time through the warp's part of the queries' memory (all products
+        // are done), so that stores are of whole sectors.
+        const unsigned long long place =
+            !is ? ~0ull : apart ? part * D : (unsigned long long)(sp.row + token) * a.out_row_stride + (unsigned long long)h * D;
+        const uint32_t stage = k.base + K::kQueries + tile * (kSplit ? 2 : 1) * K::kQueryBytes + (warp & 3) * 4096;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          uint32_t o[16];
-          if (j > 0) {
-            tmem_load16(out_at(tile) + lanes + c, o);
-            tmem_loaded();
-          }
-          if (is)
+        for (int c = 0; c < D; c += 32) {
+#pragma unroll
+          for (int half = 0; half < 32; half += 16) {
+            uint32_t o[16];
+            if (j > 0) {
+              tmem_load16(out_at(tile) + lanes + c + half, o);
+              tmem_loaded();
+            }
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-              float v[4];
+              uint32_t v[4];
 #pragma unroll
               for (int i = 0; i < 4; i++)
-                v[i] = l != 0.0f ? __uint_as_float(o[e + i]) * f : 0.0f;
-              const float4 v4 = make_float4(v[0], v[1], v[2], v[3]);
-              if (parts.splits > 1)
-                *reinterpret_cast<float4 *>(parts.o + part * D + c + e) = v4;
-              else
-                store4(a, (size_t)(sp.row + token) * a.out_row_stride + (size_t)h * D + c + e, v4);
+                v[i] = l != 0.0f ? __float_as_uint(__uint_as_float(o[e + i]) * f) : 0u;
+              K::store16(stage + lane * 128 + (((half + e) / 4 ^ (lane & 7)) << 4), v[0], v[1], v[2], v[3]);
             }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int row_here = i * 4 + (lane >> 3), piece = lane & 7;
+            const unsigned long long to = __shfl_sync(0xffffffffu, place, row_here) + c + piece * 4;
+            const bool there = __shfl_sync(0xffffffffu, (int)is, row_here);
+            const uint4 v = lds16(stage + row_here * 128 + ((piece ^ (row_here & 7)) << 4));
+            const float4 v4 = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+            if (there && apart)
+              *reinterpret_cast<float4 *>(parts.o + to) = v4;
+            else if (there)
+              store4(a, to, v4);
+          }
+          __syncwarp();
         }
       }
     }
@@ -766,10 +803,10 @@ template <typename QT> void launch_tiles(cudaStream_t stream, const Call<QT> &a,
     launch_with<QT, 128, 2>(stream, a, two, splits, workspace);
     return;
   }
-  // Four tiles fit tensor memory at 64 elements and bf16 rows (one part of weights); see the top for what they
-  // bring.  Where they would leave SMs without a block, two.
+  // Four tiles fit tensor memory at 64 elements and bf16 rows (one part of weights).  Where they would leave SMs
+  // without a block, two.  @@FOUR@@
   if constexpr (sizeof(QT) == 2)
-    if ((four - a.rows.n_seqs) * a.cache.n_kv_heads >= sm_count()) {
+    if ((four - a.rows.n_seqs) * a.cache.n_kv_heads >= sm_count() * 7 / 8) {
       launch_with<QT, 64, 4>(stream, a, four, 1, workspace);
       return;
     }
