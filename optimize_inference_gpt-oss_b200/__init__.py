@@ -257,8 +257,8 @@ class DeviceBuffer:
 
 
 def _ptr(x):
-    if x is None:
-        return None
+    if x is None or type(x) is int:  # asked first: a call has up to ten of these and is short itself
+        return x
     if hasattr(x, "ptr"):  # a DeviceBuffer, or any view object that carries a device address
         return x.ptr
     return int(x)

@@ -38,15 +38,17 @@ struct Rows {
     const int r0 = start(s), n = max(start(s + 1) - r0, 0);
     return Span{r0, min(n, max_new), min(max(__ldg(kv_len + s), 0), kMaxTokens) - n};
   }
-  // The last sequence s with first(s) <= u, where first(s) never falls as s grows and first(0) <= u.
+  // The last sequence s with first(s) <= u, where first(s) never falls as s grows and first(0) <= u.  By whole
+  // warps, 32 places looked at per round: a search by halves is a chain of loads eight long at 200 sequences.
   template <typename F> __device__ __forceinline__ int find(int u, F first) const {
-    int lo = 0, hi = n_seqs;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (first(mid) <= u)
-        lo = mid;
-      else
-        hi = mid;
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = n_seqs;
+    while (n > 1) {
+      const int step = (n + 31) / 32, at = min(lane * step, n - 1);
+      const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && first(lo + at) <= u);
+      const int k = 31 - __clz(below | 1u);
+      lo += k * step;
+      n = min(step, n - k * step);
     }
     return lo;
   }

@@ -13,8 +13,9 @@
 // then codes) so that they are read once; in a decode step, latency -- a warp per group, four
 // groups to a block, and a chain of four dependent loads (lengths, table entry, row, scale).
 //
-// Measured: 192 rows of a decode step 5 us; 11400 rows of twelve prompts (8 heads of 64: 23 MB in, 12 MB out) 17 us
-// with cold caches, 0.3 of a copy's rate: blocks of 8 KB, each a chain of dependent loads, three waves of them.
+// Measured: 192 rows of a decode step 5 us; 11400 rows of twelve prompts (8 heads of 64: 23 MB in, 12 MB out) 14 us
+// with cold caches, 0.4 of a copy's rate (19 us with a clamp and a conversion per value): blocks of 8 KB, each a chain of
+// dependent loads, two waves of them.
 #include "kv8.cuh"
 
 namespace gptoss {
@@ -41,10 +42,19 @@ template <typename QT> struct Eight; // eight stored values, as they lie in memo
 template <> struct Eight<float> {
   uint4 a, b;
   __device__ __forceinline__ Vec8 floats() const { return floats_of(a, b); }
+  // Largest |x| as bits (of an fp32 number; a NaN's are above an infinity's).
+  __device__ __forceinline__ uint32_t top() const {
+    const uint32_t m = 0x7fffffffu;
+    return max(max(max(a.x & m, a.y & m), max(a.z & m, a.w & m)), max(max(b.x & m, b.y & m), max(b.z & m, b.w & m)));
+  }
 };
 template <> struct Eight<uint16_t> {
   uint4 a;
   __device__ __forceinline__ Vec8 floats() const { return widen8(a); }
+  __device__ __forceinline__ uint32_t top() const { // two at a time
+    const uint32_t m = 0x7fff7fffu, t = __vmaxu2(__vmaxu2(a.x & m, a.y & m), __vmaxu2(a.z & m, a.w & m));
+    return max(t & 0xffff0000u, t << 16);
+  }
 };
 template <bool VEC> __device__ __forceinline__ Eight<float> load_eight(const float *p) {
   if constexpr (VEC)
@@ -62,12 +72,14 @@ template <bool VEC> __device__ __forceinline__ Eight<uint16_t> load_eight(const 
                        p[6] | (uint32_t)p[7] << 16)};
 }
 
-__device__ __forceinline__ uint32_t pack_codes(const float *v, float inverse) {
-  uint32_t r = 0;
+// Four codes.  1.5 * 2^23 leaves fp32 whole numbers, so one fused multiply-add rounds v * inverse to even
+// and its lowest byte is the code: three instructions per value where clamping and converting took twelve.
+__device__ __forceinline__ uint32_t pack_finite(const float *v, float inverse) {
+  uint32_t x[4];
 #pragma unroll
   for (int i = 0; i < 4; i++)
-    r |= ((uint32_t)__float2int_rn(v[i] * inverse) & 0xffu) << (8 * i);
-  return r;
+    x[i] = __float_as_uint(fmaf(v[i], inverse, 12582912.0f));
+  return __byte_perm(__byte_perm(x[0], x[1], 0x0040), __byte_perm(x[2], x[3], 0x0040), 0x5410);
 }
 __device__ __forceinline__ uint32_t rescale_codes(uint32_t w, float keep) {
   uint32_t r = 0;
@@ -109,7 +121,7 @@ __global__ void __launch_bounds__(128)
   src += (size_t)(n_q_heads + kind * cache.n_kv_heads + (active ? head : 0)) * D + element;
 
   Eight<QT> held[kHold ? kPasses : 1];
-  float top = 0.0f;
+  uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < kPasses; i++) {
     const int slot = (kHold ? 0 : slot0) + i * kRowsPerPass + sub;
@@ -117,24 +129,42 @@ __global__ void __launch_bounds__(128)
       const Eight<QT> e = load_eight<VEC>(src + (long)slot * row_stride);
       if constexpr (kHold)
         held[i] = e;
-      const Vec8 v = e.floats();
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-        top = fmaxf(top, fabsf(storable(v.v[j])));
+      bits = max(bits, e.top());
     }
     if (!kHold && slot0 + (i + 1) * kRowsPerPass >= slot1)
       break;
   }
+  auto group_max = [&](uint32_t x) {
+    x = __reduce_max_sync(0xffffffffu, x);
+    if constexpr (GROUP == 128) {
+      __shared__ uint32_t part[4];
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0)
+        part[threadIdx.x >> 5] = x;
+      __syncthreads();
+      x = max(max(part[0], part[1]), max(part[2], part[3]));
+    }
+    return x;
+  };
+  bits = group_max(bits);
+  const bool finite = bits < 0x7f800000u;
+  if (!finite) { // once more, with what is to be stored in place of NaN and infinities
+    bits = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if constexpr (GROUP == 128) {
-    __shared__ float part[4];
-    if ((threadIdx.x & 31) == 0)
-      part[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    for (int i = 0; i < kPasses; i++) {
+      const int slot = (kHold ? 0 : slot0) + i * kRowsPerPass + sub;
+      if (kHold ? (slot >= slot0 && slot < slot1) : slot < slot1) {
+        const Vec8 v = kHold ? held[kHold ? i : 0].floats() : load_eight<VEC>(src + (long)slot * row_stride).floats();
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          bits = max(bits, __float_as_uint(fabsf(storable(v.v[j]))));
+      }
+      if (!kHold && slot0 + (i + 1) * kRowsPerPass >= slot1)
+        break;
+    }
+    bits = group_max(bits);
   }
+  const float top = __uint_as_float(bits);
   if (!active)
     return;
 
@@ -167,10 +197,16 @@ __global__ void __launch_bounds__(128)
     const int slot = (kHold ? 0 : slot0) + i * kRowsPerPass + sub;
     if (kHold ? (slot >= slot0 && slot < slot1) : slot < slot1) {
       Vec8 v = kHold ? held[kHold ? i : 0].floats() : load_eight<VEC>(src + (long)slot * row_stride).floats();
+      uint2 codes;
+      if (finite)
+        codes = make_uint2(pack_finite(v.v, inverse), pack_finite(v.v + 4, inverse));
+      else {
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        v.v[j] = storable(v.v[j]);
-      *reinterpret_cast<uint2 *>(block + slot * D) = make_uint2(pack_codes(v.v, inverse), pack_codes(v.v + 4, inverse));
+        for (int j = 0; j < 8; j++)
+          v.v[j] = storable(v.v[j]);
+        codes = make_uint2(pack_finite(v.v, inverse), pack_finite(v.v + 4, inverse));
+      }
+      *reinterpret_cast<uint2 *>(block + slot * D) = codes;
     }
     if (!kHold && slot0 + (i + 1) * kRowsPerPass >= slot1)
       break;
