@@ -339,6 +339,88 @@ def test_attend_masked_query_does_not_leak(gpu):
         assert np.isnan(got[1, 0]).all()
 
 
+@pytest.mark.parametrize("dtype_name", ["bf16", "f32"])
+@pytest.mark.parametrize("n_q,heads,D", [(80, 1, 64), (130, 1, 128), (33, 1, 64), (400, 2, 64)])
+def test_attend_wide_groups(gpu, dtype_name, n_q, heads, D):
+    """Many query heads to one key/value head: a single token is then many rows."""
+    pkg = gpu
+    st = Step(pkg, 121 + n_q, [300, 64, 2000, 7], [1, 1, 1, 2], n_q, heads, D, pkg.BF16 if dtype_name == "bf16" else pkg.F32, trail=1).put()
+    st.check_attend(sinks=st.r.standard_normal(n_q).astype(np.float32))
+    st.check_attend(window=100, first=5)
+
+
+@pytest.mark.parametrize("n,most_new,n_q,heads", [(3000, 1, 2, 1), (1100, 3, 2, 1), (130, 10, 8, 1)])
+def test_many_sequences(gpu, n, most_new, n_q, heads):
+    """More sequences than a block has threads or a warp lanes: lengths from 0 to three pages and one long one, in a wide
+    table; row counts from 0 on (10 rows of 8 heads: the tile kernel's, 8 and fewer the token kernels')."""
+    pkg = gpu
+    r = np.random.default_rng(n)
+    lens = r.integers(0, 190, n)
+    lens[n // 2] = 1200
+    new = np.minimum(r.integers(0, most_new + 1, n), lens)
+    st = Step(pkg, n, [int(x) for x in lens], [int(x) for x in new], n_q, heads, 64, pkg.BF16, width=20).put()
+    st.append()
+    st.check_append()
+    st.codes[0], st.scales[0] = ko.append(st.codes[0], st.scales[0], st.x, n_q, st.row_start, st.kv_len, st.pages, st.max_new)
+    st.check_attend()
+    st.check_attend(window=40, first=3)
+
+
+@pytest.mark.parametrize("new", [1, 200])
+def test_offsets_past_32_bits(gpu, new):
+    """A pool of 4.6 GB, pages at both ends of it, the second of two layers."""
+    pkg = gpu
+    n_pages, heads, D, n_q, length = 35001, 8, 64, 16, 200
+    page_bytes = heads * 2 * PAGE * D
+    d = Dev(pkg)
+    codes, scales = pkg.DeviceBuffer(2 * n_pages * page_bytes), pkg.DeviceBuffer.filled(2 * n_pages * heads * 8, 0xff)
+    pool = pkg.kv8_pool(codes, scales, 2, n_pages, heads, D)
+    used = np.array([35000, 3, 17500, 34999], np.int32)
+    r = np.random.default_rng(5)
+    x = widen(pkg, r.standard_normal((length, (n_q + 2 * heads) * D)).astype(np.float32), pkg.BF16)
+    small = np.arange(4, dtype=np.int32)[None]
+    want_c, want_s = ko.append(np.zeros((4, heads, 2, PAGE, D), np.int8), np.full((4, heads, 2), np.nan, np.float32), x, n_q,
+                               [0, length], [length], small, length)
+    row = x.shape[1]
+    args = (1, length, d.put(x, pkg.BF16), pkg.BF16, row, n_q, 1, d.put(np.array([0, length], np.int32)),
+            d.put(np.array([length], np.int32)), d.put(used[None]), 4)
+    pkg.kv8_append(pool, *args, length)
+    pkg.kv8_copy_pages(pool, 1, d.put(used[:1]), d.put(np.array([34000], np.int32)))
+    for i, page in list(enumerate(used)) + [(0, 34000)]:
+        at = (n_pages + int(page))
+        got = codes.numpy(np.int8, (heads, 2, PAGE, D), at * page_bytes)
+        full = min(length - i * PAGE, PAGE)
+        assert np.array_equal(got[:, :, :full], want_c[i][:, :, :full])
+        assert_bit_equal(scales.numpy(np.float32, (heads, 2), at * heads * 8), want_s[i])
+    rows = x[length - new:]
+    n = pkg.kv8_attention_workspace(pool, new, n_q, 1, new)
+    out = d.out((new, n_q * D), pkg.BF16)
+    pkg.kv8_attention(pool, 1, new, d.put(rows, pkg.BF16), pkg.BF16, row, n_q, 1, d.put(np.array([0, new], np.int32)), *args[8:],
+                      new, 0.125, 0, 0, None, out, pkg.BF16, n_q * D, d.out((n,), np.uint8), n)
+    ref, *bounds = ko.attend(want_c, want_s, rows, n_q, [0, new], [length], small, new, 0.125, 0, 0, None)
+    assert (np.abs(out.get().reshape(new, n_q, D) - ref) <= ko.tolerance(ref, *bounds, False, False)).all()
+    codes.free()
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that overlap in time, each with its own workspace and output."""
+    pkg = gpu
+    sts = [Step(pkg, 111 + i, [4000, 900, 70], new, 16, 2, 64, pkg.BF16).put() for i, new in enumerate(([1, 1, 1], [1, 90, 30]))]
+    streams = [pkg.Stream() for _ in sts]
+    outs = [[st.dev.out((st.T, 16 * 64), pkg.BF16) for _ in range(6)] for st in sts]
+    wss = [st.attend(o[0], pkg.BF16, 0.125) for st, o in zip(sts, outs)]
+    pkg.synchronize()
+    for k in range(1, 6):
+        for st, o, ws, stream in zip(sts, outs, wss, streams):
+            st.attend(o[k], pkg.BF16, 0.125, ws=ws, stream=stream.h)
+    pkg.synchronize()
+    for o in outs:
+        for k in range(1, 6):
+            assert np.array_equal(o[0].get(as_f32=False), o[k].get(as_f32=False))
+    for stream in streams:
+        stream.close()
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1], [3, 2, 1], [70, 1, 200]])
 def test_attend_repeats_to_the_bit_and_replays(gpu, new):
     """Twice the same bits; on a stream of its own; captured and replayed with other lengths and rows;
