@@ -9,7 +9,7 @@
 //     O += P V    128 x D, P from tensor memory, values from shared memory
 // What would bound it at D = 64 is the exponential (16 per clock and SM: 512 clocks for a 128 x 64 tile against some
 // 320 of matrix instructions); what does is how far the steps of a tile, which wait for each other (scores,
-// weights, product), are covered by those of the others: 850 clocks per tile and page with four tiles, 1250 with two.
+// weights, product), are covered by those of the others: 810 clocks per tile and page with four tiles, 1230 with two.
 // An 8192-token prompt of 64 heads takes 0.79 ms, 0.70 PFLOP/s.  So:
 //   - four warps per tile: softmax.  A row's running maximum is raised only when the new one is 2^8 above it, so
 //     that O is rescaled a few times per row and not once per page;
