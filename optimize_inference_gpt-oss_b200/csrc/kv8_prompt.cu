@@ -116,25 +116,26 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
 }
 #define GPTOSS_R8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
 #define GPTOSS_W8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
-// 32 columns of the calling warp's 32 lanes; the values are there after tmem_loaded.
-__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t *x) {
+// 32 columns of the calling warp's 32 lanes; the values are there after tmem_loaded.  Arrays of another size than the
+// columns moved do not compile.
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t (&x)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
                "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                : GPTOSS_R8(x, 0), GPTOSS_R8(x, 8), GPTOSS_R8(x, 16), GPTOSS_R8(x, 24)
                : "r"(at));
 }
-__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *x) {
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&x)[32]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
                "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
                GPTOSS_W8(x, 0), GPTOSS_W8(x, 8), GPTOSS_W8(x, 16), GPTOSS_W8(x, 24)
                : "memory");
 }
-__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t *x) {
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t (&x)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                : GPTOSS_R8(x, 0), GPTOSS_R8(x, 8)
                : "r"(at));
 }
-__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t *x) {
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&x)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
                GPTOSS_W8(x, 0), GPTOSS_W8(x, 8)
                : "memory");
@@ -406,24 +407,24 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
       auto step = [&](const Meta &it, int j) {
         // All 64 scores in registers where there is room (two tiles); else half by half, and the first half again for the
         // weights, which lie where their own half's scores were.
-        constexpr int kHeld = TILES == 2 ? 64 : 32;
-        uint32_t x[kHeld];
-        tmem_load32(scores_at(tile, j) + lanes, x);
-        if constexpr (kHeld == 64)
-          tmem_load32(scores_at(tile, j) + lanes + 32, x + 32);
+        constexpr int kHalves = TILES == 2 ? 2 : 1, kHeld = 32 * kHalves; // in registers
+        uint32_t x[kHalves][32];
+#pragma unroll
+        for (int i = 0; i < kHalves; i++)
+          tmem_load32(scores_at(tile, j) + lanes + 32 * i, x[i]);
         tmem_loaded();
         float tops[4] = {-3e38f, -3e38f, -3e38f, -3e38f}; // four chains, so that none waits for itself
 #pragma unroll
         for (int c0 = 0; c0 < kPage; c0 += kHeld) {
           if (c0 > 0) {
-            tmem_load32(scores_at(tile, j) + lanes + 32, x);
+            tmem_load32(scores_at(tile, j) + lanes + 32, x[0]);
             tmem_loaded();
           }
 #pragma unroll
           for (int c = 0; c < kHeld; c += 8)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-              tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + 4 + e])));
+              tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(x[c / 32][c % 32 + e]), __uint_as_float(x[c / 32][c % 32 + 4 + e])));
         }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const bool any = top > -2e38f; // real scores are below 2^28
@@ -460,17 +461,18 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
         for (int h0 = 0; h0 < kPage; h0 += kHeld) {
           const int c0 = kHeld == 64 ? 0 : kHeld - h0; // the half that is still in registers first
           if (h0 > 0) {
-            tmem_load32(scores_at(tile, j) + lanes + c0, x);
+            tmem_load32(scores_at(tile, j) + lanes + c0, x[0]);
             tmem_loaded();
           }
 #pragma unroll
           for (int c = 0; c < kHeld; c += 2) {
-            const float2 z = fma2(make_float2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), make_float2(f, f), make_float2(off, off));
+            const float2 z = fma2(make_float2(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])),
+                                  make_float2(f, f), make_float2(off, off));
             float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
             sums[c / 2 & 3] = add2(sums[c / 2 & 3], p);
             w[c / 2] = pack_f16(p.x, p.y);
             if constexpr (kSplit)
-              x[c / 2] = pack_rest(w[c / 2], p.x, p.y); // x[c / 2] has been read
+              x[0][c / 2] = pack_rest(w[c / 2], p.x, p.y); // x[0][c / 2] has been read
           }
           if constexpr (kHeld == 64)
             tmem_store32(scores_at(tile, j) + lanes, w);
@@ -479,9 +481,8 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
         }
         const float2 sum = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
         l += sum.x + sum.y;
-        tmem_store32(scores_at(tile, j) + lanes, w);
         if constexpr (kSplit)
-          tmem_store32(scores_at(tile, j) + lanes + 32, x);
+          tmem_store32(scores_at(tile, j) + lanes + 32, x[0]);
         return true;
       };
       bool ok = true;
