@@ -453,7 +453,11 @@ GPTOSS_API int gptoss_kv8_append(gptoss_stream_t stream, const gptoss_kv8_pool_t
  * sequence are left as they were.
  * Products are taken on the tensor cores with the codes as they are (exact in fp16); fp32 rows
  * (qkv_dtype GPTOSS_F32) and the softmax weights that go with them are carried as two fp16 parts, so
- * that the result has fp32's accuracy; sums are fp32.
+ * that the result has fp32's accuracy; the weights of bf16 rows are rounded to one fp16 number (2^-11),
+ * whatever the output's type; a weight below 2^-33 of the row's largest may count as 0; sums are fp32.
+ * Pages whose value scale is more than 2^10 from that of the others are summed apart, in fp32, and
+ * joined (slower: made for pages that hardly ever are), so that a row's result does not depend on the size
+ * of values it does not see.  Scores z have to lie within fp32's range.
  * workspace: gptoss_kv8_attention_workspace bytes (for the same arguments on the same device),
  * 16-byte aligned, contents irrelevant; calls that may overlap in time need one each.
  */

@@ -13,7 +13,7 @@
 //   - the order of a head's elements within a product and of a step's tokens is free, and is chosen so
 //     that a lane needs 16 or 8 consecutive bytes of a token;
 //   - codes become fp16 exactly (kv8_mma.cuh); key scales multiply the scores, value scales, powers
-//     of two, multiply the codes relative to the largest met so far;
+//     of two, multiply the codes relative to a reference of the warp (kv8_attention.cuh, also on pages far from it);
 //   - queries are brought to fp16 range by a power of two per row; a bf16 row is then exact, an fp32 row
 //     is two fp16 parts and two products, and so are its softmax weights, which is what keeps fp32's
 //     accuracy on these tensor cores;
@@ -73,13 +73,14 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
   static constexpr int kDepth = (WHOLE ? 4096 : 8192) / kPart;
   static constexpr int kResult = kRows * (kPitch * 4 + 8); // a warp's results, which lie where its ring was
   static constexpr int kRing = 2 * kDepth * kPart > kResult ? 2 * kDepth * kPart : kResult; // 8 or 16 KB per warp
-  static constexpr int kSmem = kTokenWarps * (kRing + 2 * kDepth * 8 + kDepth * 16);
+  static constexpr int kSmem = kTokenWarps * (kRing + 2 * kDepth * 8 + kDepth * 16 + 4);
   using VWord = typename std::conditional<D == 64, uint2, uint4>::type;
 
   uint32_t q[RB][KS][2], q_rest[kSplit ? RB : 1][kSplit ? KS : 1][2];
   float row_factor[RB][2], m[RB][2], l[RB][2], o[RB][DT][4]; // of rows 2t, 2t + 1 of each 8
   int row_pos[RB][2];                                        // -1: no such row
-  int value_exp;
+  int ref;             // exponent of the value scale that this warp's outputs are relative to; 0: no page has had one yet
+  bool met_far;        // pages far from it were left out
   uint32_t ring, bars; // this warp's, as shared-space addresses
   int4 *slots;         // what a part is: page, step, scales
   int done;            // parts used so far, over all items
@@ -150,7 +151,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
   }
 
   __device__ __forceinline__ void begin() {
-    value_exp = 0;
+    ref = 0, met_far = false;
 #pragma unroll
     for (int b = 0; b < RB; b++)
 #pragma unroll
@@ -193,12 +194,10 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
 
   // s becomes the weights of the step's tokens first_token ..
   template <bool MASKED>
-  __device__ __forceinline__ void weigh(float (&s)[RB][TT][4], float key_scale, int v_exp, int first_token, int window,
-                                        int n_first) {
+  __device__ __forceinline__ void weigh(float (&s)[RB][TT][4], float key_scale, int first_token, int window, int n_first) {
     const int first = first_token + token_of((threadIdx.x & 31) >> 2); // tile i's rows g, g + 8: tokens first + 16 i, + 8
-    bool moved = v_exp > value_exp;
+    bool moved = false;
     float fade[RB][2];
-    const float beta = moved ? two_to(value_exp - v_exp) : 1.0f;
 #pragma unroll
     for (int b = 0; b < RB; b++)
 #pragma unroll
@@ -227,7 +226,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
         const float a = fast_exp2(m[b][e] - base), off = (float)kWeightBits - base;
         m[b][e] = now;
         moved = moved || a != 1.0f;
-        fade[b][e] = a * beta;
+        fade[b][e] = a;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < TT; i++)
@@ -241,7 +240,6 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
           }
         l[b][e] = fmaf(l[b][e], a, sum);
       }
-    value_exp = max(value_exp, v_exp);
     if (__any_sync(0xffffffffu, moved))
 #pragma unroll
       for (int b = 0; b < RB; b++)
@@ -254,7 +252,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
     const int lane = threadIdx.x & 31, t = lane & 3;
     const uint32_t even = values + token_of(2 * t) * D + (lane >> 2) * (D / 8), odd = values + token_of(2 * t + 1) * D + (lane >> 2) * (D / 8);
     uint32_t mul, add;
-    value_factor(v_exp == 0 ? -99 : v_exp - value_exp + kValueBits, mul, add);
+    value_factor(v_exp, ref, mul, add);
 #pragma unroll
     for (int i = 0; i < TT; i++) {
       uint32_t p[RB][2], rest[kSplit ? RB : 1][2];
@@ -370,14 +368,26 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
         break;
       }
       float w[RB][TT][4];
+      const int v_exp = exponent_field(__int_as_float(it.w));
+      ref = ref ? ref : v_exp;
+      if (is_far(v_exp, ref)) { // left to finish: its parts are given back as they are
+        met_far = true;
+        if (!arrived(done, 1)) {
+          lost = true;
+          break;
+        }
+        __syncwarp();
+        ask_keys(true);
+        continue;
+      }
       scores(w, part_at(done, 0));
       __syncwarp(); // every lane has read the keys and the slot
       ask_keys(false);
-      const int token = cols.at(it.y / kSteps) * kPage + (it.y % kSteps) * CH, v_exp = exponent_field(__int_as_float(it.w));
+      const int token = cols.at(it.y / kSteps) * kPage + (it.y % kSteps) * CH;
       if (token + CH - 1 <= min_pos && (a.window <= 0 || token > max_pos - a.window || token + CH <= a.n_first))
-        weigh<false>(w, __int_as_float(it.z), v_exp, token, a.window, a.n_first);
+        weigh<false>(w, __int_as_float(it.z), token, a.window, a.n_first);
       else
-        weigh<true>(w, __int_as_float(it.z), v_exp, token, a.window, a.n_first);
+        weigh<true>(w, __int_as_float(it.z), token, a.window, a.n_first);
       if (!arrived(done, 1)) {
         lost = true;
         break;
@@ -395,14 +405,18 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
     }
   }
 
-  // The warps' results joined: into the output, or into a piece for merge_pieces.  Whole block.
-  __device__ __forceinline__ void finish(const Call<QT> &a, const Rows::Span &sp, int head, int row0, float *piece_o,
-                                         float2 *piece_ml) {
+  // The warps' results, and the far pages of columns [i0, i1), joined: into the output, or into a piece for
+  // merge_pieces.  Whole block.
+  __device__ __forceinline__ void finish(const Call<QT> &a, const Rows::Span &sp, int s, int head, int row0, const Columns &cols,
+                                         int i0, int i1, float *piece_o, float2 *piece_ml) {
     extern __shared__ __align__(16) uint8_t smem[];
     auto so = [&](int w, int r) { return reinterpret_cast<float *>(smem + w * kRing) + r * kPitch; };
     auto sml = [&](int w) { return reinterpret_cast<float2 *>(smem + w * kRing + kRows * kPitch * 4); };
+    int *const refs = reinterpret_cast<int *>(smem + kTokenWarps * (kRing + 2 * kDepth * 8 + kDepth * 16)); // the warps'
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const float unit = two_to(value_exp - 127 - kValueBits);
+    const float unit = two_to(ref - 127);
+    if (lane == 0)
+      refs[warp] = ref;
 #pragma unroll
     for (int b = 0; b < RB; b++)
 #pragma unroll
@@ -414,14 +428,15 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
         const int r = 8 * b + 2 * t + e;
         if (g == 0)
           sml(warp)[r] = make_float2(m[b][e], sum * two_to(-kWeightBits));
-        const float f = sum > 0.0f ? unit / sum : 0.0f;
+        const float f = sum > 0.0f ? (float)(1 << (kNear - kValueBits)) / sum : 0.0f;
         float *row = so(warp, r) + g * (D / 8);
+        auto mean = [&](float x) { return finite(x * f * unit); }; // 64 x 2^122 is not; a NaN shows by its sum
 #pragma unroll
         for (int j = 0; j < DT; j += 2)
           *reinterpret_cast<float4 *>(row + 2 * j) =
-              make_float4(o[b][j][e] * f, o[b][j][2 + e] * f, o[b][j + 1][e] * f, o[b][j + 1][2 + e] * f);
+              make_float4(mean(o[b][j][e]), mean(o[b][j][2 + e]), mean(o[b][j + 1][e]), mean(o[b][j + 1][2 + e]));
       }
-    __syncthreads();
+    const bool far = __syncthreads_or(met_far);
     const int R = min(sp.q * a.group - row0, kRows);
     for (int i = threadIdx.x; i < R * (D / 4); i += kTokenWarps * 32) {
       const int r = i / (D / 4), d = (i % (D / 4)) * 4, h = head * a.group + (row0 + r) % a.group;
@@ -435,19 +450,30 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
         top = fmaxf(top, ml[w].x);
       }
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (far) {
+        const int token = (row0 + r) / a.group;
+        const QT *q = a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D;
+        const FarSum<4> fs = far_pages<D, 4>(a, s, cols, i0, i1, head, q, sp.pos + token, d, refs, kTokenWarps, kSteps);
+        top = fmaxf(top, fs.m);
+        const float f = fs.l != 0.0f ? fast_exp2(fs.m - top) : 0.0f;
+        sum = fs.l * f;
+        acc = make_float4(fs.o[0] * f, fs.o[1] * f, fs.o[2] * f, fs.o[3] * f);
+      }
 #pragma unroll
       for (int w = 0; w < kTokenWarps; w++) {
         const float part = ml[w].y != 0.0f ? ml[w].y * fast_exp2(ml[w].x - top) : 0.0f; // a NaN passes
         const float4 x = *reinterpret_cast<const float4 *>(so(w, r) + d);
+        const float of = part * two_to(-kSumBits);
         sum += part;
-        acc.x += part * x.x, acc.y += part * x.y, acc.z += part * x.z, acc.w += part * x.w;
+        acc.x += of * x.x, acc.y += of * x.y, acc.z += of * x.z, acc.w += of * x.w;
       }
       if (sink && sum != 0.0f)
         sum += fast_exp2(z - top);
-      const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
+      const float f = sum != 0.0f ? (float)(1 << kSumBits) / sum : 0.0f;
       acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
       if (piece_o) {
-        *reinterpret_cast<float4 *>(piece_o + (size_t)r * D + d) = acc;
+        *reinterpret_cast<float4 *>(piece_o + (size_t)r * D + d) =
+            make_float4(finite(acc.x), finite(acc.y), finite(acc.z), finite(acc.w));
         if (d == 0)
           piece_ml[r] = make_float2(top, sum);
       } else {
@@ -462,7 +488,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
   __device__ __forceinline__ void item(const Call<QT> &a, const Rows::Span &sp, int s, int head, int rg, const Columns &cols,
                                        int i0, int i1, int min_pos, int max_pos, float *piece_o, float2 *piece_ml) {
     run(a, sp, s, head, rg * kRows, cols, i0, i1, min_pos, max_pos);
-    finish(a, sp, head, rg * kRows, piece_o, piece_ml);
+    finish(a, sp, s, head, rg * kRows, cols, i0, i1, piece_o, piece_ml);
   }
 };
 
@@ -477,7 +503,7 @@ __device__ __forceinline__ GroupRange group_range(const Rows::Span &sp, int grou
 // items' columns, in order, in equal pieces.
 template <typename QT, int D, int RB, bool WHOLE>
 __global__ void __launch_bounds__(kTokenWarps * 32, RB <= 2 ? (WHOLE && D == 64 && RB == 1 ? 4 : 3) : 2)
-    attend_tokens(Call<QT> a, int above, int upto, int groups, Pieces pieces) { // sequences of above < rows <= upto
+    attend_tokens(const __grid_constant__ Call<QT> a, int above, int upto, int groups, Pieces pieces) { // sequences of above < rows <= upto
   using K = TokenKernel<QT, D, RB, WHOLE>;
   pdl_prologue();
   K k;
@@ -618,9 +644,9 @@ template <typename QT, int D, int RB> __global__ void __launch_bounds__(kMergeTh
     for (int b = blockIdx.x + slice; b <= it.w; b += slices) {
       const float2 ml = pieces.ml[slot(b)];
       const float4 x = *reinterpret_cast<const float4 *>(pieces.o + slot(b) * D + d);
-      const float part = ml.y != 0.0f ? ml.y * fast_exp2(ml.x - top) : 0.0f;
+      const float part = ml.y != 0.0f ? ml.y * fast_exp2(ml.x - top) : 0.0f, of = part * two_to(-kSumBits);
       sum += part;
-      acc.x += part * x.x, acc.y += part * x.y, acc.z += part * x.z, acc.w += part * x.w;
+      acc.x += of * x.x, acc.y += of * x.y, acc.z += of * x.z, acc.w += of * x.w;
     }
   part_of[threadIdx.x] = acc, sum_of[threadIdx.x] = sum;
   __syncthreads();
@@ -633,7 +659,7 @@ template <typename QT, int D, int RB> __global__ void __launch_bounds__(kMergeTh
   }
   if (sum != 0.0f && a.sinks)
     sum += fast_exp2(z - top);
-  const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
+  const float f = sum != 0.0f ? (float)(1 << kSumBits) / sum : 0.0f;
   store4(a, (size_t)(sp.row + row / a.group) * a.out_row_stride + (size_t)h * D + d,
          make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
 }

@@ -8,7 +8,13 @@ namespace gptoss {
 namespace kv8 {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kValueBits = 5;     // codes of the largest value scale met so far are held times 2^5
+// Value scales.  Codes are multiplied by their page's scale relative to a reference, the scale of the first page that
+// has one: by 2^(kValueBits - 2 kNear) to 2^kValueBits, exact in fp16, for scales within 2^kNear of the reference.  Pages
+// further away (far pages: one value 1000 times its neighbours', an infinity stored as the largest finite number) are left
+// out there and summed by far_pages, in fp32, row by row, and only then joined: what a row holds never depends on the
+// size of what it does not see, or gives no weight.  (A reference that followed the largest page lost everything 2^29
+// smaller, for all rows of a block; one per row would still lose it where the large code is not the row's to see.)
+constexpr int kNear = 10, kValueBits = 5;
 constexpr int kMaxTokenRows = 64; // (new tokens) x (query heads per key/value head) of one sequence: attend_tokens up to
                                   // here, attend_tiles above (24 sequences of 40 rows and 2000 tokens: 57 us here, 77
                                   // there; of 64 rows 84 and 86; 100 of 64 rows and 1000 tokens 211 and 145; one of 64
@@ -42,12 +48,17 @@ __device__ __forceinline__ Columns columns(const Rows &rows, int window, int n_f
   return Columns{head, lo, head + last - lo + 1};
 }
 
-// fp16 2^e and -1152 * 2^e, twice in a word; e <= 5, zero below fp16's range.
-__device__ __forceinline__ void value_factor(int e, uint32_t &mul, uint32_t &add) {
-  const uint32_t m = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
-  const uint32_t a = e >= -24 ? 0x8080u | (uint32_t)(e + 25) << 10 : 0u;
-  mul = m * 0x10001u, add = a * 0x10001u;
+__device__ __forceinline__ bool is_far(int v_exp, int ref) { return v_exp != 0 && (unsigned)(v_exp - ref + kNear) > 2u * kNear; }
+// fp16 2^e and -1152 * 2^e, twice in a word, for the values of a page that is not far (e in [-15, 5]); zero for a page of
+// zeros.
+__device__ __forceinline__ void value_factor(int v_exp, int ref, uint32_t &mul, uint32_t &add) {
+  const int e = v_exp - ref - kNear + kValueBits;
+  const uint32_t m = e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << 9, a = 0x8080u | (uint32_t)(e + 25) << 10;
+  mul = v_exp ? m * 0x10001u : 0u, add = v_exp ? a * 0x10001u : 0u;
 }
+// Where weighted values are added up before the division they are held in units of 2^kSumBits: a few thousand of 2^128.
+constexpr int kSumBits = 16;
+__device__ __forceinline__ float finite(float x) { return fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f); }
 
 template <typename QT> __device__ __forceinline__ void load4(const QT *p, bool vec, float (&v)[4]) {
   if (vec) {
@@ -79,6 +90,85 @@ template <typename QT> __device__ __forceinline__ void store4(const Call<QT> &a,
     else
       store1(p, v.x), store1(p + 1, v.y), store1(p + 2, v.z), store1(p + 3, v.w);
   }
+}
+
+// What one row (query q at position pos) sees of the far pages among the columns [i0, i1): maximum, sum of the weights,
+// and N of its elements from d0 on, in units of 2^kSumBits.  A page is `steps` steps, dealt in turn to n_refs warps; refs
+// has the references they held pages against.  Plain fp32, eight tokens at a time: some ten times what a near page costs,
+// for pages that hardly ever are.  A call of its own, so that it takes no registers from the kernels' loops (inlined,
+// prompts ran 2-3 % longer).
+template <int N> struct FarSum {
+  float m, l, o[N];
+};
+template <int D, int N, typename QT>
+__device__ __noinline__ FarSum<N> far_pages(const Call<QT> &a, int s, Columns cols, int i0, int i1, int head, const QT *q, int pos,
+                                            int d0, const int *refs, int n_refs, int steps) {
+  const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
+  FarSum<N> f;
+  f.m = -INFINITY, f.l = 0.0f;
+#pragma unroll
+  for (int n = 0; n < N; n++)
+    f.o[n] = 0.0f;
+  bool odd = false;
+#pragma unroll 1
+  for (int d = 0; d < D; d++)
+    odd = odd || !(fabsf(load1(q + d)) <= 3.402823466e38f);
+#pragma unroll 1
+  for (int i = i0; i < i1; i++) {
+    const int page = a.cache.checked(__ldg(table + cols.at(i)));
+    if (page < 0)
+      continue;
+    const float *scale = a.cache.scale(page, head);
+    const int v_exp = exponent_field(scale[1]);
+    const int8_t *block = a.cache.template block<D>(page, head);
+    const float factor = odd ? NAN : a.scale * kLog2e * scale[0], unit = two_to(v_exp - 127 - kSumBits);
+#pragma unroll 1
+    for (int t0 = 0; t0 < kPage; t0 += 8) {
+      if (!is_far(v_exp, refs[((i - i0) * steps + t0 * steps / kPage) % n_refs]))
+        continue;
+      float z[8], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int token = cols.at(i) * kPage + t0 + u;
+        z[u] = -INFINITY;
+        if (token <= pos && (a.window <= 0 || token > pos - a.window || token < a.n_first)) {
+          float part[4] = {};
+#pragma unroll 1
+          for (int d = 0; d < D; d += 4) {
+            const char4 k = *reinterpret_cast<const char4 *>(block + (t0 + u) * D + d);
+            float x[4];
+            load4(q + d, a.q_vec, x);
+            part[0] = fmaf(x[0] * factor, k.x, part[0]), part[1] = fmaf(x[1] * factor, k.y, part[1]);
+            part[2] = fmaf(x[2] * factor, k.z, part[2]), part[3] = fmaf(x[3] * factor, k.w, part[3]);
+          }
+          z[u] = (part[0] + part[1]) + (part[2] + part[3]);
+        }
+        top = fmaxf(top, z[u]);
+      }
+      const float now = fmaxf(f.m, top), base = now > -INFINITY ? now : 0.0f, fade = fast_exp2(f.m - base);
+      float sum = 0.0f;
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        z[u] = fast_exp2(z[u] - base);
+        sum += z[u];
+      }
+      f.m = now, f.l = fmaf(f.l, fade, sum);
+#pragma unroll
+      for (int n = 0; n < N; n += 4) {
+        float part[4] = {};
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const char4 v = *reinterpret_cast<const char4 *>(block + (kPage + t0 + u) * D + d0 + n);
+          part[0] = fmaf(z[u], v.x, part[0]), part[1] = fmaf(z[u], v.y, part[1]);
+          part[2] = fmaf(z[u], v.z, part[2]), part[3] = fmaf(z[u], v.w, part[3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          f.o[n + e] = fmaf(f.o[n + e], fade, part[e] * unit);
+      }
+    }
+  }
+  return f;
 }
 
 // Sequences of more than kMaxTokenRows rows (kv8_prompt.cu).

@@ -209,10 +209,10 @@ template <typename QT, int D, int TILES> struct TileKernel {
   }
 };
 
-struct Meta { // of a page: its first token (-1: there are no more), key scale, the exponent values are relative to
+struct Meta { // of a page: its first token, key scale; behind the last (token -1) the value reference, and if there are far pages
   int token;
   float key_scale;
-  int value_exp, unused;
+  int ref, far;
 };
 
 // The `rows` rows of a sequence and head that a block works on, and the table columns they look at.  Units are
@@ -250,7 +250,7 @@ struct Parts {
 };
 
 template <typename QT, int D, int TILES>
-__global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT> a, Parts parts) {
+__global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __grid_constant__ Call<QT> a, Parts parts) {
   using K = TileKernel<QT, D, TILES>;
   constexpr bool kSplit = K::kSplit;
   constexpr int kBuffers = K::kBuffers, kLeader = 32 * K::kConverters; // kLeader: the thread that asks for pages
@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
         arrive_warp(k.bar(K::kQueryFull));
       }
       float m = -INFINITY, l = 0.0f;
-      int value_exp = 0, j = 0;
+      int j = 0, ref = 0;
+      bool far = false;
       // What this thread's row does not see of a page gets a score below all others.  Only pages at the edge of
       // what a tile sees come here, and the step itself has one form: with the masks in it, it ran 13 % longer
       // over the pages that need none.
@@ -432,12 +433,10 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
         float f = row_factor * it.key_scale;
         f = any ? (f < 0x1p-100f ? 0x1p-100f : f) : 1.0f;
         const float now = any ? fmaxf(m, top * f) : m;
-        if (__any_sync(0xffffffffu, now > m + kRise || it.value_exp != value_exp)) {
+        if (__any_sync(0xffffffffu, now > m + kRise)) {
           const float fade = now > -INFINITY ? fast_exp2(m - now) : 1.0f;
-          const float factor = fade * two_to(value_exp - it.value_exp);
           m = now;
           l *= fade;
-          value_exp = it.value_exp;
           if (j > 0) {
             if (!k.wait_warp(K::kOutDone + tile, (j - 1) & 1))
               return false;
@@ -449,7 +448,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
               tmem_loaded();
 #pragma unroll
               for (int e = 0; e < 16; e++)
-                o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
               tmem_store16(out_at(tile) + lanes + c, o);
             }
           }
@@ -491,8 +490,10 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
           break;
         tc_after_sync();
         const Meta it = meta[j % kMeta];
-        if (it.token < 0)
+        if (it.token < 0) {
+          ref = it.ref, far = it.far;
           break;
+        }
         const bool all = it.token + kPage - 1 <= min_pos &&
                          (a.window <= 0 || it.token > max_pos - a.window || it.token + kPage <= a.n_first);
         if (!all)
@@ -507,56 +508,88 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
         ok = k.wait_warp(K::kOutDone + tile, (j - 1) & 1);
       if (ok) {
         tc_after_sync();
-        float f = 0.0f;
-        if (l != 0.0f) { // a NaN passes
-          const bool sink = parts.splits == 1 && a.sinks;
-          const float z = sink ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY, top = fmaxf(m, z);
-          const float fade = m > -INFINITY ? fast_exp2(m - top) : 1.0f;
-          const float all = l * fade + (sink ? fast_exp2(z - top + (float)kTileBits) : 0.0f);
-          f = fade * two_to(value_exp - 127 - kValueBits) / all;
-        }
         const bool apart = parts.splits > 1;
+        const float z = !apart && a.sinks ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY;
+        // What the tiles' sums and those of the row's far pages (maximum and sum there) are multiplied by; what a part leaves.
+        float f = 0.0f, f_far = 0.0f;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        auto share = [&](float m_far, float l_far) {
+          if (l == 0.0f && l_far == 0.0f) // a NaN passes
+            return;
+          const float top = fmaxf(fmaxf(m, m_far), z);
+          const float fade = l != 0.0f ? (m > -INFINITY ? fast_exp2(m - top) : 1.0f) * two_to(-kTileBits) : 0.0f;
+          const float fade_far = l_far != 0.0f ? (m_far > -INFINITY ? fast_exp2(m_far - top) : 1.0f) : 0.0f;
+          const float seen = l * fade + l_far * fade_far, all = seen + fast_exp2(z - top);
+          f = fade * (float)(1 << (kNear - kValueBits)) / all, f_far = fade_far * (float)(1 << kSumBits) / all;
+          ml = make_float2(top, seen);
+        };
+        share(-INFINITY, 0.0f);
         const size_t part = (size_t)blockIdx.x * K::kRowsOfBlock + tile * kTile + r;
-        if (apart && is)
-          parts.ml[part] = make_float2(m, l * two_to(-kTileBits));
         // Where the row goes; then 32 elements at a time through the warp's part of the queries' memory (all products
         // are done), so that stores are of whole sectors.
         const unsigned long long place =
             !is ? ~0ull : apart ? part * D : (unsigned long long)(sp.row + token) * a.out_row_stride + (unsigned long long)h * D;
         const uint32_t stage = k.base + K::kQueries + tile * (kSplit ? 2 : 1) * K::kQueryBytes + (warp & 3) * 4096;
+        auto write = [&](auto with_far) {
+          constexpr bool kFar = decltype(with_far)::value;
+          const float unit = two_to(ref - 127);
+          Unit v = {}; // for far pages, found again: nothing that only they need is held over the pages
+          if constexpr (kFar)
+            (void)v.find(a, (int)(gridDim.x / parts.splits / heads) - 1 - index / heads, index % heads, K::kRowsOfBlock);
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+          for (int c = 0; c < D; c += 32) {
 #pragma unroll
-          for (int half = 0; half < 32; half += 16) {
-            uint32_t o[16];
-            if (j > 0) {
-              tmem_load16(out_at(tile) + lanes + c + half, o);
-              tmem_loaded();
+            for (int half = 0; half < 32; half += 16) {
+              FarSum<16> fs = {};
+              if constexpr (kFar) {
+                if (is) {
+                  fs = far_pages<D, 16>(a, v.s, v.cols, v.column(split, parts.splits), v.column(split + 1, parts.splits), v.head,
+                                        a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D, pos, c + half,
+                                        &meta[j % kMeta].ref, 1, 1);
+                  share(fs.m, fs.l); // every time the same
+                }
+                __syncwarp();
+              }
+              uint32_t o[16];
+              if (j > 0) {
+                tmem_load16(out_at(tile) + lanes + c + half, o);
+                tmem_loaded();
+              }
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) {
+                uint32_t v4[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                  float x = l != 0.0f ? __uint_as_float(o[e + i]) * f * unit : 0.0f;
+                  if constexpr (kFar)
+                    x = fmaf(fs.o[e + i], f_far, x);
+                  v4[i] = __float_as_uint(kFar && apart ? finite(x) : x); // a part's NaN shows by its sum
+                }
+                K::store16(stage + lane * 128 + (((half + e) / 4 ^ (lane & 7)) << 4), v4[0], v4[1], v4[2], v4[3]);
+              }
             }
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              uint32_t v[4];
-#pragma unroll
-              for (int i = 0; i < 4; i++)
-                v[i] = l != 0.0f ? __float_as_uint(__uint_as_float(o[e + i]) * f) : 0u;
-              K::store16(stage + lane * 128 + (((half + e) / 4 ^ (lane & 7)) << 4), v[0], v[1], v[2], v[3]);
+            for (int i = 0; i < 8; i++) {
+              const int row_here = i * 4 + (lane >> 3), piece = lane & 7;
+              const unsigned long long to = __shfl_sync(0xffffffffu, place, row_here) + c + piece * 4;
+              const bool there = __shfl_sync(0xffffffffu, (int)is, row_here);
+              const uint4 w = lds16(stage + row_here * 128 + ((piece ^ (row_here & 7)) << 4));
+              const float4 w4 = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+              if (there && apart)
+                *reinterpret_cast<float4 *>(parts.o + to) = w4;
+              else if (there)
+                store4(a, to, w4);
             }
+            __syncwarp();
           }
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int row_here = i * 4 + (lane >> 3), piece = lane & 7;
-            const unsigned long long to = __shfl_sync(0xffffffffu, place, row_here) + c + piece * 4;
-            const bool there = __shfl_sync(0xffffffffu, (int)is, row_here);
-            const uint4 v = lds16(stage + row_here * 128 + ((piece ^ (row_here & 7)) << 4));
-            const float4 v4 = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-            if (there && apart)
-              *reinterpret_cast<float4 *>(parts.o + to) = v4;
-            else if (there)
-              store4(a, to, v4);
-          }
-          __syncwarp();
-        }
+        };
+        if (far)
+          write(std::true_type{});
+        else
+          write(std::false_type{});
+        if (apart && is)
+          parts.ml[part] = ml;
       }
     }
   } else if (warp < K::kIssuer) {
@@ -565,8 +598,9 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
     const int t = threadIdx.x & 63;
     const bool values = warp >= K::kConverters + 2;
     const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
-    int page_of = -1, held = col0 - 32, asked = 0, value_exp = 0;
-    unsigned there = 0; // of the columns held .. held + 31: those with a page that is still to be asked for
+    int page_of = -1, held = col0 - 32, asked = 0, ref = 0; // ref: exponent of the first value scale there is
+    bool any_far = false;
+    unsigned there = 0; // of the columns held .. held + 31: those with a page, not a far one, that is still to be asked for
     float2 scale_of = make_float2(0.0f, 0.0f);
     // Every warp goes over the table the same way; one thread asks for the bytes.  Per raw stage:
     int ring_token[K::kRawStages];
@@ -578,7 +612,13 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
         page_of = held + lane < col1 ? a.cache.checked(__ldg(table + cols.at(held + lane))) : -1;
         if (page_of >= 0)
           scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
-        there = __ballot_sync(0xffffffffu, page_of >= 0);
+        const int v_exp = page_of >= 0 ? exponent_field(scale_of.y) : 0;
+        const unsigned valued = __ballot_sync(0xffffffffu, v_exp != 0);
+        if (ref == 0 && valued)
+          ref = __shfl_sync(0xffffffffu, v_exp, __ffs(valued) - 1);
+        const unsigned far = __ballot_sync(0xffffffffu, is_far(v_exp, ref));
+        any_far = any_far || far;
+        there = __ballot_sync(0xffffffffu, page_of >= 0) & ~far;
       }
       if (!there)
         return;
@@ -632,17 +672,14 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(Call<QT>
           break;
         if (j >= K::kRawStages && !(ok = k.wait_warp((values ? K::kValueFree : K::kKeyFree) + stage, turn ^ 1)))
           break;
-        const int v_exp = exponent_field(ring_scale[stage].y);
-        if (more)
-          value_exp = max(value_exp, v_exp);
-        if (threadIdx.x == kLeader)
-          meta[j % kMeta] = Meta{ring_token[stage], ring_scale[stage].x, value_exp, 0};
+        if (threadIdx.x == kLeader) // behind the last page all columns have been looked at
+          meta[j % kMeta] = Meta{ring_token[stage], ring_scale[stage].x, ref, any_far};
         if (more) {
           if (!(ok = k.wait_warp(K::kRawFull + stage, turn)))
             break;
           uint32_t mul = 0x3c003c00u, add = 0xe480e480u; // times 1, minus 1152
           if (values)
-            value_factor(v_exp == 0 ? -99 : v_exp - value_exp + kValueBits, mul, add);
+            value_factor(exponent_field(ring_scale[stage].y), ref, mul, add);
           convert(k.base + K::kRaw + stage * K::kRawBytes + (values ? kPage * D : 0),
                   k.base + (values ? K::kValues : K::kKeys) + stage * K::kPageBytes, mul, add);
         }
@@ -762,13 +799,13 @@ template <typename QT, int D> __global__ void __launch_bounds__(256) merge_parts
     if (u.column(i, parts.splits) < u.column(i + 1, parts.splits)) {
       const float2 ml = parts.ml[at(i)];
       const float4 x = *reinterpret_cast<const float4 *>(parts.o + at(i) * D + d);
-      const float part = ml.y != 0.0f ? ml.y * fast_exp2(ml.x - top) : 0.0f; // a NaN passes
+      const float part = ml.y != 0.0f ? ml.y * fast_exp2(ml.x - top) : 0.0f, of = part * two_to(-kSumBits); // a NaN passes
       sum += part;
-      acc.x += part * x.x, acc.y += part * x.y, acc.z += part * x.z, acc.w += part * x.w;
+      acc.x += of * x.x, acc.y += of * x.y, acc.z += of * x.z, acc.w += of * x.w;
     }
   if (sum != 0.0f && a.sinks)
     sum += fast_exp2(z - top);
-  const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
+  const float f = sum != 0.0f ? (float)(1 << kSumBits) / sum : 0.0f;
   store4(a, (size_t)(u.sp.row + (u.row0 + r) / a.group) * a.out_row_stride + (size_t)h * D + d,
          make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
 }

@@ -1,0 +1,177 @@
+"""The 8-bit paged cache where its definition is easy to lose: values of very different size, numbers that
+are none.  Every form of the attention (rows per sequence, type, how the work is shared out) takes the same
+cases."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import kv8_oracle as ko
+from gpu_util import widen
+from test_gpu_kv8 import PAGE, Step
+
+pytestmark = pytest.mark.gpu
+
+# name: lengths, new rows, query heads, key/value heads, head_dim, types
+FORMS = {
+    "tokens": ([333, 64, 700], [1, 1, 1], 8, 2, 64, ("bf16", "f32")),
+    "tokens of wide heads": ([333, 700], [1, 1], 16, 2, 128, ("bf16", "f32")),
+    "pieces of a long one": ([9000, 130], [1, 1], 8, 1, 64, ("bf16", "f32")),
+    "16 rows": ([333, 700], [4, 2], 8, 2, 64, ("bf16", "f32")),
+    "some rows": ([333, 640, 90], [13, 7, 1], 8, 2, 64, ("bf16", "f32")),
+    "two tiles": ([300, 333], [300, 90], 8, 2, 64, ("bf16", "f32")),
+    "two tiles of wide heads": ([300, 333], [300, 90], 8, 2, 128, ("bf16", "f32")),
+    "columns shared out": ([3000, 200], [40, 30], 16, 2, 64, ("bf16", "f32")),
+    "four tiles": ([700, 500, 5], [700, 430, 1], 64, 8, 64, ("bf16",)),
+}
+every_form = pytest.mark.parametrize("form,dtype_name", [(f, t) for f, v in FORMS.items() for t in v[5]])
+
+
+def step_of(pkg, form, dtype_name, seed, **kw):
+    lens, new, n_q, heads, D, _ = FORMS[form]
+    return Step(pkg, seed, lens, new, n_q, heads, D, pkg.BF16 if dtype_name == "bf16" else pkg.F32, trail=2, **kw)
+
+
+def run(st, out_dtype, scale=0.125, window=0, first=0, sinks=None):
+    pkg = st.pkg
+    out = st.dev.out((st.T, st.n_q * st.D), out_dtype)
+    ws = st.attend(out, out_dtype, scale, window, first, st.dev.put(sinks) if sinks is not None else None)
+    got = out.get().reshape(st.T, st.n_q, st.D)
+    ws.get()
+    assert pkg.load().gptoss_wait_giveups() == 0
+    return got
+
+
+def want(st, scale=0.125, window=0, first=0, sinks=None):
+    """The definition in 64 bits, and per (row, head) what errors scale with: sum p |v|, the largest
+    scale * sum |q k|, the tokens seen; and what fp16 weights may lose.  A row's weights are fp16 numbers of which
+    the largest is at least 2^7, so that each is rounded by at most 2^-25, or 2^-32 of the largest, and by
+    no more than itself."""
+    codes, scales = st.codes[st.layer].astype(np.float64), st.scales[st.layer].astype(np.float64)
+    T, n_q, D, G = st.T, st.n_q, st.D, st.n_q // st.heads
+    x = st.x.reshape(T, -1, D)[:, :n_q].astype(np.float64)
+    out, weight, grain = np.full((T, n_q, D), np.nan), np.zeros((T, n_q, D)), np.zeros((T, n_q, D))
+    reach, seen = np.zeros((T, n_q, 1)), np.zeros((T, n_q, 1))
+    for s, r0, q, pos in ko.spans(st.row_start, st.kv_len, T, st.max_new):
+        t = np.array([i for i in range(max(pos + q, 0)) if ko.page_of(st.pages, s, i, codes.shape[0]) >= 0], np.int64)
+        if not q:
+            continue
+        pg, slot, p = st.pages[s, t // PAGE] if len(t) else t, t % PAGE, pos + np.arange(q)[:, None]
+        ok = t[None] <= p
+        if window > 0:
+            ok &= (t[None] > p - window) | (t[None] < first)
+        any_ = ok.any(1, keepdims=True)
+        for h in range(n_q):
+            g, r = h // G, slice(r0, r0 + q)
+            k, v = (codes[pg, g, i, slot] * scales[pg, g, i][:, None] for i in (0, 1))
+            z = np.where(ok, scale * (x[r, h] @ k.T), -np.inf)
+            sink = -np.inf if sinks is None else float(sinks[h])
+            top = np.maximum(z.max(1, initial=-np.inf, keepdims=True), sink)
+            top = np.where(np.isfinite(top), top, 0.0)
+            w = np.exp(z - top)
+            w = w / np.where(any_, w.sum(1, keepdims=True) + np.exp(sink - top), 1.0)
+            out[r, h], weight[r, h] = w @ v, w @ np.abs(v)
+            grain[r, h] = np.minimum(w, w.max(1, initial=0, keepdims=True) * 2.0 ** -32) @ np.abs(v)
+            reach[r, h] = np.where(ok, np.abs(x[r, h]) @ np.abs(k.T), 0).max(1, initial=0, keepdims=True) * abs(scale)
+            seen[r, h] = ok.sum(1, keepdims=True)
+    return out, weight, reach, seen, grain
+
+
+def check(st, got, ref, weight, reach, seen, grain, out_dtype, rows=None):
+    """ko.tolerance's shares, element by element, with `grain` for its term of the largest value."""
+    pkg = st.pkg
+    tol = ko.tolerance(ref, weight, reach, seen, np.zeros_like(seen), st.dtype == pkg.F32, out_dtype == pkg.F32) + grain
+    there = ~np.isnan(ref).any((1, 2))
+    if rows is not None:
+        there &= rows
+    err, tol = np.abs(got.astype(np.float64) - ref)[there], tol[there]
+    assert np.isfinite(got[there]).all(), "not finite"
+    assert (err <= tol).all(), f"{int((err > tol).sum())} of {err.size} off; worst {np.max(err / tol):.3g} of the bound"
+
+
+# ---- values of very different size ---------------------------------------------------------
+
+
+@every_form
+def test_values_of_pages_far_apart(gpu, form, dtype_name):
+    """Value scales from 2^-60 to 2^60, pages of zeros among them, scores that differ by some tens: a small
+    page counts where the large ones weigh nothing, or are not seen."""
+    st = step_of(gpu, form, dtype_name, 201)
+    st.x[:, :st.n_q * st.D] *= 4
+    st.x = widen(gpu, st.x, st.dtype)
+    st.scales[..., 1] = 2.0 ** st.r.integers(-60, 61, st.scales.shape[:-1])
+    st.scales[0, st.pages[0, 1], 0, 1] = 0
+    st.put()
+    sinks = st.r.standard_normal(st.n_q).astype(np.float32)
+    for kw in (dict(), dict(window=100, first=3, sinks=sinks), dict(window=64, scale=-0.125)):
+        check(st, run(st, gpu.F32, **kw), *want(st, **kw), gpu.F32)
+
+
+@every_form
+@pytest.mark.parametrize("window", [0, 70])
+def test_an_infinite_value_shows_only_where_it_is_seen(gpu, form, dtype_name, window):
+    """One value as append stores an infinity (64 x 2^122, all others of its page 0), among ordinary ones:
+    rows before it, and rows whose window has passed it, do not know of it."""
+    st = step_of(gpu, form, dtype_name, 211)
+    for s in range(len(st.kv_len)):
+        n = int(st.kv_len[s])
+        t = max(n - 40 if n - 40 < n - st.max_new // 2 else n - st.max_new // 2, 0) if window == 0 else max(n - 85, 0)
+        page = st.pages[s, t // PAGE]
+        st.scales[0, page, :, 1], st.codes[0, page, :, 1] = 2.0 ** 122, 0
+        st.codes[0, page, :, 1, t % PAGE, 3] = 64
+    st.put()
+    ref = want(st, window=window)
+    check(st, run(st, gpu.F32, window=window), *ref, gpu.F32)
+    out = run(st, gpu.BF16, window=window)
+    sane = (np.abs(ref[0]) < 1e30).all((1, 2)) & ~np.isnan(ref[0]).any((1, 2))
+    if st.max_new > 60 or window:
+        assert sane.any()
+    check(st, out, *ref, gpu.BF16, sane)
+
+
+@every_form
+def test_a_huge_value_that_weighs_nothing(gpu, form, dtype_name):
+    """Every row sees a token whose value is 2^60 times the others' and whose weight is some 2^-70 or less."""
+    st = step_of(gpu, form, dtype_name, 221)
+    n = st.n_q * st.D
+    st.x[:, :n] = np.abs(st.x[:, :n])
+    st.x = widen(gpu, st.x, st.dtype)
+    for s in range(len(st.kv_len)):
+        page = st.pages[s, 0]
+        st.codes[0, page, :, 0, 0], st.scales[0, page, :, 0] = -127, 2.0 ** -3
+        st.codes[0, page, :, 0, 1:] //= 4
+        st.scales[0, page, :, 1] = 2.0 ** 57
+        st.codes[0, page, :, 1, 1:] = 0
+    st.put()
+    check(st, run(st, gpu.F32), *want(st), gpu.F32)
+
+
+# ---- what is not a number -----------------------------------------------------------------
+
+
+
+@every_form
+def test_queries_that_are_not_numbers_show_in_their_own_rows(gpu, form, dtype_name):
+    """NaN and infinities in single query heads give NaN there and show nowhere else, also where the row's
+    context is cut and joined; a row that sees nothing gives 0 all the same."""
+    st = step_of(gpu, form, dtype_name, 241)
+    clean = st.x.copy()
+    last, D = int(st.row_start[-1]) - 1, st.D
+    bad = {(0, 0): np.nan, (last, 1): np.inf, (last // 2, st.n_q - 1): -np.inf}
+    for (r, h), value in bad.items():
+        st.x[r, h * D + 5] = value
+        clean[r, h * D + 5] = 0
+    st.put()
+    got = run(st, gpu.F32)
+    st.x = clean
+    ref = want(st)
+    for r, h in bad:
+        assert np.isnan(got[r, h]).all(), (r, h)
+        got[r, h] = ref[0][r, h]
+    check(st, got, *ref, gpu.F32)
+    st = step_of(gpu, form, dtype_name, 242)
+    st.pages[:] = -1
+    st.x[:, 7] = np.nan
+    st.put()
+    got = run(st, gpu.F32, sinks=np.zeros(st.n_q, np.float32))
+    assert (got[:st.row_start[-1]] == 0).all()
