@@ -447,8 +447,8 @@ GPTOSS_API int gptoss_kv8_append(gptoss_stream_t stream, const gptoss_kv8_pool_t
  * A row sees t <= p, and with window > 0 only t > p - window or t < n_first (the first tokens stay
  * visible); tokens without a page are not seen by anybody.  sinks (fp32, one logit per query head,
  * may be NULL) takes part in the denominator only (run.cpp:611-636 of the reference).  Where nothing
- * is seen the output is 0; otherwise a query head with a NaN or an infinity in it gives NaN, and
- * shows in no other output.  window 0 means no window.  Query head h reads key/value head
+ * is seen the output is 0; otherwise a query head with a NaN or an infinity in it, or a NaN for its sink
+ * logit, gives NaN, and shows in no other output.  window 0 means no window.  Query head h reads key/value head
  * h / (n_q_heads / n_kv_heads).  out has n_q_heads * head_dim values per row; rows that belong to no
  * sequence are left as they were.
  * Products are taken on the tensor cores with the codes as they are (exact in fp16); fp32 rows

@@ -441,7 +441,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
     for (int i = threadIdx.x; i < R * (D / 4); i += kTokenWarps * 32) {
       const int r = i / (D / 4), d = (i % (D / 4)) * 4, h = head * a.group + (row0 + r) % a.group;
       const bool sink = !piece_o && a.sinks;
-      const float z = sink ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY;
+      const float z = sink ? sink_of(a, h) : -INFINITY;
       float2 ml[kTokenWarps];
       float top = z, sum = 0.0f;
 #pragma unroll
@@ -633,7 +633,7 @@ template <typename QT, int D, int RB> __global__ void __launch_bounds__(kMergeTh
   const int r = row0 + i / D4, d = (i % D4) * 4;
   const int row = it.z * kRows + r, h = it.y * a.group + row % a.group;
   auto slot = [&](int b) { return ((size_t)b * 2 + (b == (int)blockIdx.x)) * kRows + r; };
-  const float z = a.sinks ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY;
+  const float z = a.sinks ? sink_of(a, h) : -INFINITY;
   float top = z, sum = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8

@@ -35,6 +35,13 @@ template <typename QT> struct Call {
   bool out_f32, q_vec, out_vec; // vec: rows may be read / written 4 elements at a time
 };
 
+// A head's sink logit in powers of two; an infinite one is brought to where differences are still numbers.  A NaN stays
+// one: no maximum takes it, but the sum does.
+template <typename QT> __device__ __forceinline__ float sink_of(const Call<QT> &a, int h) {
+  const float z = __ldg(a.sinks + h) * kLog2e;
+  return z > 3e38f ? 3e38f : z;
+}
+
 // The table columns a row group looks at: the first `head` ones, then those from `lo` on; n in all (at
 // least one, so that every row is visited; what it must not see is masked).
 struct Columns {

@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
       if (ok) {
         tc_after_sync();
         const bool apart = parts.splits > 1;
-        const float z = !apart && a.sinks ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY;
+        const float z = !apart && a.sinks ? sink_of(a, h) : -INFINITY;
         // What the tiles' sums and those of the row's far pages (maximum and sum there) are multiplied by; what a part leaves.
         float f = 0.0f, f_far = 0.0f;
         float2 ml = make_float2(-INFINITY, 0.0f);
@@ -786,7 +786,7 @@ template <typename QT, int D> __global__ void __launch_bounds__(256) merge_parts
   if (!u.find(a, (int)(gridDim.x / heads) - 1 - index / heads, index % heads, rows) || u.row0 + r >= u.R)
     return;
   const int d = threadIdx.x % D4 * 4, h = u.head * a.group + (int)((u.row0 + r) % a.group);
-  const float z = a.sinks ? fminf(__ldg(a.sinks + h) * kLog2e, 3e38f) : -INFINITY;
+  const float z = a.sinks ? sink_of(a, h) : -INFINITY;
   auto at = [&](int split) { return ((size_t)index * parts.splits + split) * rows + r; };
   float top = z, sum = 0.0f;
 #pragma unroll 8

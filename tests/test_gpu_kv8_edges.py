@@ -1,6 +1,6 @@
-"""The 8-bit paged cache where its definition is easy to lose: values of very different size, numbers that
-are none.  Every form of the attention (rows per sequence, type, how the work is shared out) takes the same
-cases."""
+"""The 8-bit paged cache where its definition is easy to lose: values of very different size, sink
+logits and queries that are not numbers, scales at the ends of fp32, tables with holes.  Every form of
+the attention (rows per sequence, type, how the work is shared out) takes the same cases."""
 from __future__ import annotations
 
 import numpy as np
@@ -148,6 +148,24 @@ def test_a_huge_value_that_weighs_nothing(gpu, form, dtype_name):
 
 # ---- what is not a number -----------------------------------------------------------------
 
+
+@every_form
+def test_a_sink_that_is_not_a_number_shows(gpu, form, dtype_name):
+    """In its own head, in every row that sees something; a row that sees nothing stays 0."""
+    st = step_of(gpu, form, dtype_name, 231)
+    st.pages[0, :] = -1
+    st.put()
+    sinks = st.r.standard_normal(st.n_q).astype(np.float32)
+    sinks[0], sinks[-1] = np.inf, np.nan
+    got = run(st, gpu.F32, sinks=sinks)
+    one = slice(st.row_start[0], st.row_start[1])
+    rest = slice(st.row_start[1], st.row_start[-1])
+    assert (got[one] == 0).all()
+    assert np.isnan(got[rest, -1]).all() and (got[rest, 0] == 0).all()
+    with np.errstate(invalid="ignore"):
+        ref = want(st, sinks=np.where(np.isfinite(sinks), sinks, 0).astype(np.float32))
+    for h in (slice(1, st.n_q - 1),):
+        check(st, got[:, h], *(a[:, h] for a in ref), gpu.F32)
 
 
 @every_form
