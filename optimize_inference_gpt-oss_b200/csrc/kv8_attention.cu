@@ -220,7 +220,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1)
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float f = row_factor[b][e] * key_scale;
+        const float f = at_most(row_factor[b][e] * key_scale, kMostFactor);
         const float now = top > -INFINITY ? fmaxf(m[b][e], top * f) : m[b][e];
         const float base = now > -INFINITY ? now : 0.0f;
         const float a = fast_exp2(m[b][e] - base), off = (float)kWeightBits - base;

@@ -42,6 +42,21 @@ template <typename QT> __device__ __forceinline__ float sink_of(const Call<QT> &
   return z > 3e38f ? 3e38f : z;
 }
 
+// Between two bounds; a NaN stays one.
+__device__ __forceinline__ float at_most(float x, float top) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(top));
+  return r;
+}
+__device__ __forceinline__ float at_least(float x, float bottom) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(bottom));
+  return r;
+}
+// A row's and a page's scale together stay finite: in a page whose key scale is 2^122 for the sake of a token that is not
+// seen the codes of the others are 0, and so are their scores.
+constexpr float kMostFactor = 3e38f;
+
 // The table columns a row group looks at: the first `head` ones, then those from `lo` on; n in all (at
 // least one, so that every row is visited; what it must not see is masked).
 struct Columns {
@@ -145,8 +160,11 @@ __device__ __noinline__ FarSum<N> far_pages(const Call<QT> &a, int s, Columns co
             const char4 k = *reinterpret_cast<const char4 *>(block + (t0 + u) * D + d);
             float x[4];
             load4(q + d, a.q_vec, x);
-            part[0] = fmaf(x[0] * factor, k.x, part[0]), part[1] = fmaf(x[1] * factor, k.y, part[1]);
-            part[2] = fmaf(x[2] * factor, k.z, part[2]), part[3] = fmaf(x[3] * factor, k.w, part[3]);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              x[e] = at_least(at_most(x[e] * factor, kMostFactor), -kMostFactor);
+            part[0] = fmaf(x[0], k.x, part[0]), part[1] = fmaf(x[1], k.y, part[1]);
+            part[2] = fmaf(x[2], k.z, part[2]), part[3] = fmaf(x[3], k.w, part[3]);
           }
           z[u] = (part[0] + part[1]) + (part[2] + part[3]);
         }

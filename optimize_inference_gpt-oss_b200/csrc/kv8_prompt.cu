@@ -430,8 +430,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const bool any = top > -2e38f; // real scores are below 2^28
         // A factor that is not 0, so that what is masked stays below; 2^-100 of a score is as good as 0.
-        float f = row_factor * it.key_scale;
-        f = any ? (f < 0x1p-100f ? 0x1p-100f : f) : 1.0f;
+        const float f = any ? at_least(at_most(row_factor * it.key_scale, kMostFactor), 0x1p-100f) : 1.0f;
         const float now = any ? fmaxf(m, top * f) : m;
         if (__any_sync(0xffffffffu, now > m + kRise)) {
           const float fade = now > -INFINITY ? fast_exp2(m - now) : 1.0f;

@@ -193,3 +193,22 @@ def test_queries_that_are_not_numbers_show_in_their_own_rows(gpu, form, dtype_na
     st.put()
     got = run(st, gpu.F32, sinks=np.zeros(st.n_q, np.float32))
     assert (got[:st.row_start[-1]] == 0).all()
+
+
+@every_form
+def test_an_infinite_key_that_is_not_seen(gpu, form, dtype_name):
+    """A page whose key scale is 2^122 for the sake of a token behind the rows (guessed and given up): the
+    others' codes in it are 0, and large queries times them are still 0."""
+    st = step_of(gpu, form, dtype_name, 251)
+    n = st.n_q * st.D
+    st.x[:, :n] *= np.float32(2.0 ** 24)
+    st.x = widen(gpu, st.x, st.dtype)
+    st.kv_len[:] = np.where(st.kv_len % PAGE == 0, st.kv_len - 1, st.kv_len)
+    for s in range(len(st.kv_len)):
+        last = int(st.kv_len[s])
+        page = st.pages[s, last // PAGE]
+        st.pages[s, :last // PAGE] = -1
+        st.scales[0, page, :, 0], st.codes[0, page, :, 0] = 2.0 ** 122, 0
+        st.codes[0, page, :, 0, last % PAGE:, 2] = 64
+    st.put()
+    check(st, run(st, gpu.F32), *want(st), gpu.F32)
