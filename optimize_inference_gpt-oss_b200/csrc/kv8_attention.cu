@@ -721,8 +721,8 @@ void launch(cudaStream_t stream, int D, const Layer &cache, const void *qkv, lon
             const Rows &rows, float scale, int window, int n_first, const float *sinks, void *out, gptoss_dtype_t out_dtype,
             long out_row_stride, void *workspace) {
   const size_t q4 = 4 * sizeof(QT), out4 = 4 * dtype_size(out_dtype);
-  const Call<QT> a = {cache, static_cast<const QT *>(qkv), row_stride, n_q_heads, n_q_heads / cache.n_kv_heads, rows, scale,
-                      window, n_first, sinks, out, out_row_stride, wait_giveups_word(), out_dtype == GPTOSS_F32,
+  const Call<QT> a = {cache, static_cast<const QT *>(qkv), row_stride, n_q_heads / cache.n_kv_heads, rows, scale, window,
+                      n_first, sinks, out, out_row_stride, wait_giveups_word(), out_dtype == GPTOSS_F32,
                       (reinterpret_cast<uintptr_t>(qkv) & (q4 - 1)) == 0 && row_stride % 4 == 0,
                       (reinterpret_cast<uintptr_t>(out) & (out4 - 1)) == 0 && out_row_stride % 4 == 0};
   if (!a.q_vec || !a.out_vec)
@@ -767,7 +767,7 @@ extern "C" int gptoss_kv8_attention(gptoss_stream_t stream, const gptoss_kv8_poo
   if (n_q_heads <= 0 || !out || out_row_stride < (long)n_q_heads * D ||
       (reinterpret_cast<uintptr_t>(out) & (dtype_size(out_dtype) - 1)))
     return GPTOSS_ERR_BAD_ARG;
-  if (n_q_heads % pool->n_kv_heads != 0 || (n_q_heads + 3) / 4 > 65535)
+  if (n_q_heads % pool->n_kv_heads != 0)
     return GPTOSS_ERR_UNSUPPORTED;
   if (!workspace || !aligned16(workspace) ||
       workspace_bytes < gptoss_kv8_attention_workspace(pool, T, n_q_heads, n_seqs, max_new))

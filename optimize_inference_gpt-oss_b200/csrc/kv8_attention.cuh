@@ -24,7 +24,7 @@ template <typename QT> struct Call {
   Layer cache;
   const QT *qkv;
   long row_stride;
-  int n_q_heads, group;
+  int group;
   Rows rows;
   float scale;
   int window, n_first;

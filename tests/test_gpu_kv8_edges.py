@@ -212,3 +212,23 @@ def test_an_infinite_key_that_is_not_seen(gpu, form, dtype_name):
         st.codes[0, page, :, 0, last % PAGE:, 2] = 64
     st.put()
     check(st, run(st, gpu.F32), *want(st), gpu.F32)
+
+
+# ---- arguments ---------------------------------------------------------------------------------
+
+
+def test_very_many_query_heads(gpu):
+    """More query heads than a grid's second dimension, all on one key/value head."""
+    pkg = gpu
+    n_q, D, length = 262144, 64, 100
+    st = Step(pkg, 261, [length], [1], n_q, 1, D, pkg.BF16).put()
+    got = run(st, pkg.BF16)[0]
+    k, v = (st.codes[0, st.pages[0, np.arange(length) // PAGE], 0, i, np.arange(length) % PAGE].astype(np.float64)
+            * st.scales[0, st.pages[0, np.arange(length) // PAGE], 0, i][:, None] for i in (0, 1))
+    x = st.x[0, :n_q * D].reshape(n_q, D).astype(np.float64)
+    z = 0.125 * x @ k.T
+    w = np.exp(z - z.max(1, keepdims=True))
+    w /= w.sum(1, keepdims=True)
+    reach = 0.125 * (np.abs(x) @ np.abs(k.T)).max(1, keepdims=True)
+    tol = ko.tolerance(w @ v, w @ np.abs(v), reach, float(length), np.abs(v).max(), False, False)
+    assert (np.abs(got - w @ v) <= tol).all()
