@@ -737,8 +737,8 @@ void launch(cudaStream_t stream, int D, const Layer &cache, const void *qkv, lon
 extern "C" size_t gptoss_kv8_attention_workspace(const gptoss_kv8_pool_t *pool, int T, int n_q_heads, int n_seqs,
                                                  int max_new) {
   using namespace gptoss;
-  if (kv8::check_pool(pool) != GPTOSS_OK || T <= 0 || n_q_heads <= 0 || n_seqs <= 0 || max_new <= 0 ||
-      n_q_heads % pool->n_kv_heads)
+  if (kv8::check_pool(pool) != GPTOSS_OK || T <= 0 || T > kv8::kMaxTokens || n_q_heads <= 0 || n_seqs <= 0 ||
+      n_seqs > kv8::kMaxTokens / 4 || max_new <= 0 || n_q_heads % pool->n_kv_heads)
     return 0;
   const int group = n_q_heads / pool->n_kv_heads;
   const size_t pieces = kv8::Pieces::bytes(sm_count() * kv8::kMostBlocksPerSm, 32, pool->head_dim);

@@ -232,3 +232,11 @@ def test_very_many_query_heads(gpu):
     reach = 0.125 * (np.abs(x) @ np.abs(k.T)).max(1, keepdims=True)
     tol = ko.tolerance(w @ v, w @ np.abs(v), reach, float(length), np.abs(v).max(), False, False)
     assert (np.abs(got - w @ v) <= tol).all()
+
+
+def test_workspace_of_calls_that_are_refused(gpu):
+    pkg = gpu
+    pool = pkg.kv8_pool(0x1000, 0x1000, 1, 10, 8, 64)
+    ws = pkg.kv8_attention_workspace
+    assert ws(pool, 1 << 30, 64, 2, 1) > 0
+    assert ws(pool, (1 << 30) + 1, 64, 2, 1) == 0 and ws(pool, 4, 64, (1 << 28) + 1, 1) == 0 and ws(pool, 4, 12, 2, 1) == 0
