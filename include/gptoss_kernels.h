@@ -495,7 +495,9 @@ GPTOSS_API int gptoss_kv8_release(gptoss_stream_t stream, int n, const int *seqs
  * Gives n listed sequences the pages for their tokens kv_len .. new_len - 1 that have none yet
  * (kv_len itself is the caller's to advance).  All or nothing per request: request i is served if
  * the free pages suffice for it and all (valid) requests listed before it.  Not served: a sequence that
- * was listed before, new_len beyond the table's width.
+ * was listed before, new_len beyond the table's width, a sequence that grows and whose last page is begun
+ * but not there (its tokens are gone; a free page in their place would hold another sequence's).  n is at
+ * most n_seqs.
  */
 GPTOSS_API int gptoss_kv8_reserve(gptoss_stream_t stream, int n, const int *seqs, const int *new_len,
                                   int n_seqs, const int *kv_len, int *pages, int pages_stride,

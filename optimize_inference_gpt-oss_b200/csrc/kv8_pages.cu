@@ -147,6 +147,12 @@ __global__ void __launch_bounds__(256) release_pages(Table t, int n, const int *
 
 // ---- reserve --------------------------------------------------------------------------
 
+// A sequence whose next token belongs on a page that it has begun and that is not there any more.  It gets none: the
+// tokens before would come back with what a free page holds, another sequence's.
+__device__ __forceinline__ bool lost_its_page(const Table &t, int s, long len) {
+  return len % kPage != 0 && !t.is_page(t.row(s)[len / kPage]);
+}
+
 // Requests 1024 at a time: columns [lo, hi) of a sequence's row that are to have pages, flattened so
 // that the threads share the columns of one long request as well as those of many short ones.
 template <typename Column>
@@ -159,7 +165,7 @@ __device__ void for_columns(const Table &t, int n, const int *seqs, const int *n
       s = seqs[i];
       if (t.has(s) && mark[s] == i) {
         const long len = max(t.kv_len[s], 0), want = new_len[i];
-        if (want <= (long)t.stride * kPage && want > len)
+        if (want <= (long)t.stride * kPage && want > len && !lost_its_page(t, s, len))
           lo = (int)((len + kPage - 1) / kPage), hi = (int)((want + kPage - 1) / kPage);
       }
     }
@@ -229,8 +235,9 @@ __global__ void __launch_bounds__(kThreads)
   if (served)
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const int s = seqs[i];
+      const long len = t.has(s) ? max(t.kv_len[s], 0) : 0;
       served[i] = t.has(s) && ws.mark[s] == i && new_len[i] <= (long)t.stride * kPage &&
-                  (ws.a[i] <= found || ws.a[i] == ws.b[i]);
+                  (ws.a[i] <= found || ws.a[i] == ws.b[i]) && (new_len[i] <= len || !lost_its_page(t, s, len));
     }
 }
 

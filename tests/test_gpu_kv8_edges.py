@@ -8,7 +8,7 @@ import pytest
 
 import kv8_oracle as ko
 from gpu_util import widen
-from test_gpu_kv8 import PAGE, Step
+from test_gpu_kv8 import PAGE, Step, Table
 
 pytestmark = pytest.mark.gpu
 
@@ -240,3 +240,22 @@ def test_workspace_of_calls_that_are_refused(gpu):
     ws = pkg.kv8_attention_workspace
     assert ws(pool, 1 << 30, 64, 2, 1) > 0
     assert ws(pool, (1 << 30) + 1, 64, 2, 1) == 0 and ws(pool, 4, 64, (1 << 28) + 1, 1) == 0 and ws(pool, 4, 12, 2, 1) == 0
+
+
+# ---- tables with holes ----------------------------------------------------------------------------
+
+
+def test_reserve_refuses_a_sequence_whose_begun_page_is_gone(gpu):
+    """Its next token has no place, and a free page in place of the lost one would show what another
+    sequence left there.  Nobody else is held up; who asks for no token is served."""
+    t = Table(gpu, 41, [70, 130, 64, 10, 64], 6, 20, share=False)
+    t.pages[0, 1], t.pages[1, 2], t.pages[3, 0] = -1, -5, 20
+    t.refs = np.bincount(t.pages[(t.pages >= 0) & (t.pages < 20)], minlength=20).astype(np.int32)
+    t.put()
+    free = np.flatnonzero(t.refs == 0)
+    served = t.dev.out((5,), np.int32)
+    gpu.kv8_reserve(5, t.ints([0, 3, 2, 1, 4]), t.ints([71, 200, 64, 130, 129]), *t.table, served, *t.ws)
+    assert served.get().tolist() == [0, 0, 1, 1, 1]
+    pages, refs = t.pages.copy(), t.refs.copy()
+    pages[4, 1:3], refs[free[:2]] = free[:2], 1
+    assert np.array_equal(t.d_pages.get(), pages) and np.array_equal(t.d_refs.get(), refs)
