@@ -190,7 +190,7 @@ __device__ void for_columns(const Table &t, int n, const int *seqs, const int *n
             up = mid;
         }
         entry = t.row(of[k]) + low[k] + (c - first[k]);
-        open = *entry < 0;
+        open = !t.is_page(*entry);
       }
       column(base + k, entry, open, c < total && c == first[k], c < total && c + 1 == first[k + 1]);
     }
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     if (ok)
       for (int j = lane; j < t.stride; j += 32)
-        ok = ok && t.row(c)[j] < 0;
+        ok = ok && !t.is_page(t.row(c)[j]);
     ok = __all_sync(0xffffffffu, ok);
     if (lane == 0)
       ws.a[i] = !ok ? 0 : len % kPage && t.is_page(t.row(p)[len / kPage]) ? 2 : 1;

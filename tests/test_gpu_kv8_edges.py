@@ -259,3 +259,24 @@ def test_reserve_refuses_a_sequence_whose_begun_page_is_gone(gpu):
     pages, refs = t.pages.copy(), t.refs.copy()
     pages[4, 1:3], refs[free[:2]] = free[:2], 1
     assert np.array_equal(t.d_pages.get(), pages) and np.array_equal(t.d_refs.get(), refs)
+
+
+def test_entries_outside_the_pool_are_no_pages(gpu):
+    """A table entry of n_pages or more means that there is no page, as a negative one does: reserve fills
+    it, and a sequence that has only such entries can become a child."""
+    t = Table(gpu, 43, [70, 0, 0, 64], 5, 20, share=False)
+    t.pages[1] = [20, -7, 1 << 30, 99, -1]
+    t.pages[3, 1:3] = [21, -3]
+    t.put()
+    free = np.flatnonzero(t.refs == 0)
+    served = t.dev.out((1,), np.int32)
+    gpu.kv8_reserve(1, t.ints([3]), t.ints([192]), *t.table, served, *t.ws)
+    assert served.get().tolist() == [1]
+    assert t.d_pages.get()[3].tolist() == [t.pages[3, 0], free[0], free[1], -1, -1]
+    served = t.dev.out((1,), np.int32)
+    gpu.kv8_fork(t.pool, 1, t.ints([0]), t.ints([1]), *t.table, served, *t.ws)
+    assert served.get().tolist() == [1]
+    pages, refs = t.d_pages.get(), t.d_refs.get()
+    assert pages[1, 0] == t.pages[0, 0] and pages[1, 1] == free[2] and refs[pages[1, 0]] == 2 and refs[free[2]] == 1
+    assert t.d_len.get()[1] == 70
+    assert all(not 0 <= p < 20 for p in pages[1, 2:])
