@@ -497,7 +497,7 @@ GPTOSS_API int gptoss_kv8_release(gptoss_stream_t stream, int n, const int *seqs
  * the free pages suffice for it and all (valid) requests listed before it.  Not served: a sequence that
  * was listed before, new_len beyond the table's width, a sequence that grows and whose last page is begun
  * but not there (its tokens are gone; a free page in their place would hold another sequence's).  n is at
- * most n_seqs.
+ * most n_seqs, and n x pages_stride at most 2^30 (GPTOSS_ERR_UNSUPPORTED above).
  */
 GPTOSS_API int gptoss_kv8_reserve(gptoss_stream_t stream, int n, const int *seqs, const int *new_len,
                                   int n_seqs, const int *kv_len, int *pages, int pages_stride,

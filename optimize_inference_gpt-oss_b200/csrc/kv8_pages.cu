@@ -482,6 +482,8 @@ extern "C" int gptoss_kv8_reserve(gptoss_stream_t stream, int n, const int *seqs
     return GPTOSS_ERR_BAD_ARG;
   if (const int st = kv8::check_table(n_seqs, pages, pages_stride, n_pages, refs))
     return st;
+  if ((long)n * pages_stride > kv8::kMaxTokens) // columns are numbered in 32 bits
+    return GPTOSS_ERR_UNSUPPORTED;
   if (n == 0)
     return GPTOSS_OK;
   if (!seqs || !new_len || !kv_len)
