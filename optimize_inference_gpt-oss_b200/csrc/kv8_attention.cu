@@ -369,7 +369,10 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
       }
       float w[RB][TT][4];
       const int v_exp = exponent_field(__int_as_float(it.w));
-      ref = ref ? ref : v_exp;
+      if (ref == 0) {
+        ref = pick_ref(page_of >= 0 ? exponent_field(scale_of.y) : 0);
+        ref = ref ? ref : v_exp; // where the lanes are on to pages without a scale
+      }
       if (is_far(v_exp, ref)) { // left to finish: its parts are given back as they are
         met_far = true;
         if (!arrived(done, 1)) {
@@ -436,8 +439,15 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
           *reinterpret_cast<float4 *>(row + 2 * j) =
               make_float4(mean(o[b][j][e]), mean(o[b][j][2 + e]), mean(o[b][j + 1][e]), mean(o[b][j + 1][2 + e]));
       }
-    const bool far = __syncthreads_or(met_far);
     const int R = min(sp.q * a.group - row0, kRows);
+    if (__syncthreads_or(met_far)) { // a row's far pages go to the result of the warp that sums them
+      for (int r = warp; r < R; r += kTokenWarps) {
+        const int token = (row0 + r) / a.group;
+        const QT *row = a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)(head * a.group + (row0 + r) % a.group) * D;
+        far_row<D>(a, s, head, cols, i0, i1, row, sp.pos + token, refs, kTokenWarps, kSteps, so(warp, r), sml(warp) + r);
+      }
+      __syncthreads();
+    }
     for (int i = threadIdx.x; i < R * (D / 4); i += kTokenWarps * 32) {
       const int r = i / (D / 4), d = (i % (D / 4)) * 4, h = head * a.group + (row0 + r) % a.group;
       const bool sink = !piece_o && a.sinks;
@@ -450,15 +460,6 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
         top = fmaxf(top, ml[w].x);
       }
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (far) {
-        const int token = (row0 + r) / a.group;
-        const QT *q = a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D;
-        const FarSum<4> fs = far_pages<D, 4>(a, s, cols, i0, i1, head, q, sp.pos + token, d, refs, kTokenWarps, kSteps);
-        top = fmaxf(top, fs.m);
-        const float f = fs.l != 0.0f ? fast_exp2(fs.m - top) : 0.0f;
-        sum = fs.l * f;
-        acc = make_float4(fs.o[0] * f, fs.o[1] * f, fs.o[2] * f, fs.o[3] * f);
-      }
 #pragma unroll
       for (int w = 0; w < kTokenWarps; w++) {
         const float part = ml[w].y != 0.0f ? ml[w].y * fast_exp2(ml[w].x - top) : 0.0f; // a NaN passes

@@ -8,10 +8,10 @@ namespace gptoss {
 namespace kv8 {
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Value scales.  Codes are multiplied by their page's scale relative to a reference, the scale of the first page that
-// has one: by 2^(kValueBits - 2 kNear) to 2^kValueBits, exact in fp16, for scales within 2^kNear of the reference.  Pages
+// Value scales.  Codes are multiplied by their page's scale relative to a reference, the scale that most of the first 32
+// pages are near: by 2^(kValueBits - 2 kNear) to 2^kValueBits, exact in fp16, for scales within 2^kNear of the reference.  Pages
 // further away (far pages: one value 1000 times its neighbours', an infinity stored as the largest finite number) are left
-// out there and summed by far_pages, in fp32, row by row, and only then joined: what a row holds never depends on the
+// out there and summed by far_row, in fp32, row by row, and only then joined: what a row holds never depends on the
 // size of what it does not see, or gives no weight.  (A reference that followed the largest page lost everything 2^29
 // smaller, for all rows of a block; one per row would still lose it where the large code is not the row's to see.)
 constexpr int kNear = 10, kValueBits = 5;
@@ -71,11 +71,24 @@ __device__ __forceinline__ Columns columns(const Rows &rows, int window, int n_f
 }
 
 __device__ __forceinline__ bool is_far(int v_exp, int ref) { return v_exp != 0 && (unsigned)(v_exp - ref + kNear) > 2u * kNear; }
+// The reference of up to 32 pages, whose value scales' exponents (0: none) the lanes have: the first's, unless most are
+// far from it and fewer from the first of those, as when the first page holds one huge value.
+__device__ __forceinline__ int pick_ref(int v_exp) {
+  const unsigned valued = __ballot_sync(0xffffffffu, v_exp != 0);
+  if (!valued)
+    return 0;
+  const int first = __shfl_sync(0xffffffffu, v_exp, __ffs(valued) - 1);
+  const unsigned far = __ballot_sync(0xffffffffu, is_far(v_exp, first));
+  if (2 * __popc(far) <= __popc(valued))
+    return first;
+  const int second = __shfl_sync(0xffffffffu, v_exp, __ffs(far) - 1);
+  return __popc(__ballot_sync(0xffffffffu, is_far(v_exp, second))) < __popc(far) ? second : first;
+}
 // fp16 2^e and -1152 * 2^e, twice in a word, for the values of a page that is not far (e in [-15, 5]); zero for a page of
 // zeros.
 __device__ __forceinline__ void value_factor(int v_exp, int ref, uint32_t &mul, uint32_t &add) {
   const int e = v_exp - ref - kNear + kValueBits;
-  const uint32_t m = e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << 9, a = 0x8080u | (uint32_t)(e + 25) << 10;
+  const uint32_t m = e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24), a = 0x8080u | (uint32_t)(e + 25) << 10;
   mul = v_exp ? m * 0x10001u : 0u, add = v_exp ? a * 0x10001u : 0u;
 }
 // Where weighted values are added up before the division they are held in units of 2^kSumBits: a few thousand of 2^128.
@@ -114,86 +127,135 @@ template <typename QT> __device__ __forceinline__ void store4(const Call<QT> &a,
   }
 }
 
-// What one row (query q at position pos) sees of the far pages among the columns [i0, i1): maximum, sum of the weights,
-// and N of its elements from d0 on, in units of 2^kSumBits.  A page is `steps` steps, dealt in turn to n_refs warps; refs
-// has the references they held pages against.  Plain fp32, eight tokens at a time: some ten times what a near page costs,
-// for pages that hardly ever are.  A call of its own, so that it takes no registers from the kernels' loops (inlined,
-// prompts ran 2-3 % longer).
-template <int N> struct FarSum {
-  float m, l, o[N];
-};
-template <int D, int N, typename QT>
-__device__ __noinline__ FarSum<N> far_pages(const Call<QT> &a, int s, Columns cols, int i0, int i1, int head, const QT *q, int pos,
-                                            int d0, const int *refs, int n_refs, int steps) {
+// What a row (query q at position pos) sees of the far pages among the columns [i0, i1), joined to what it saw of the
+// others: `mean` (D values) and ml (maximum, sum of the weights), both in shared memory.  A page is `steps` steps, dealt in
+// turn to n_refs warps; refs has the references they held pages against.  Plain fp32 by a whole warp, two tokens to a lane
+// for the scores, then D / 32 elements: made for pages that hardly ever are.  One such page in each of 64 sequences of
+// 8000 tokens: 0.12 -> 0.23 ms; in a prompt of 2048 tokens 0.10 -> 0.49.  A call of its own, so that it takes no registers
+// from the kernels' loops.
+template <int D, typename QT>
+__device__ __noinline__ void far_row(const Call<QT> &a, int s, int head, Columns cols, int i0, int i1, const QT *q, int pos,
+                                     const int *refs, int n_refs, int steps, float *mean, float2 *ml) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
   const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
-  FarSum<N> f;
-  f.m = -INFINITY, f.l = 0.0f;
-#pragma unroll
-  for (int n = 0; n < N; n++)
-    f.o[n] = 0.0f;
+  auto value = [](uint32_t w, int i) { // byte i of four biased codes: the lowest of 2^23 + code + 128
+    return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | i)) - 8388736.0f;
+  };
+  float top = 0.0f;
   bool odd = false;
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    const float x = load1(q + lane * N + n);
+    odd = odd || !(fabsf(x) <= 3.402823466e38f);
+    top = fmaxf(top, fabsf(x));
+  }
+  odd = __any_sync(0xffffffffu, odd);
+  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+  const int up = odd || top == 0.0f ? 0 : max(min(127 - exponent_field(top), 126), -126); // largest |q| into [1, 2)
+  const float lift = two_to(up), row_factor = odd ? NAN : a.scale * kLog2e * two_to(-up);
+  float m = -INFINITY, l = 0.0f, o[N] = {};
+  int page_of = -1, held = i0 - 32; // lane l has the page and scales of column held + l
+  float2 scale_of = make_float2(0.0f, 0.0f);
+  unsigned far = 0; // columns with a far page that are still to be done
 #pragma unroll 1
-  for (int d = 0; d < D; d++)
-    odd = odd || !(fabsf(load1(q + d)) <= 3.402823466e38f);
-#pragma unroll 1
-  for (int i = i0; i < i1; i++) {
-    const int page = a.cache.checked(__ldg(table + cols.at(i)));
-    if (page < 0)
+  for (;;) {
+    while (!far && held + 32 < i1) {
+      held += 32;
+      const int i = held + lane;
+      page_of = i < i1 ? a.cache.checked(__ldg(table + cols.at(i))) : -1;
+      bool any = false;
+      if (page_of >= 0) {
+        scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
+        for (int step = 0; step < steps; step++)
+          any = any || is_far(exponent_field(scale_of.y), refs[((i - i0) * steps + step) % n_refs]);
+      }
+      far = __ballot_sync(0xffffffffu, any);
+    }
+    if (!far)
+      break;
+    const int from = __ffs(far) - 1, i = held + from, page = __shfl_sync(0xffffffffu, page_of, from);
+    far &= far - 1;
+    const float key_scale = __shfl_sync(0xffffffffu, scale_of.x, from);
+    const int v_exp = exponent_field(__shfl_sync(0xffffffffu, scale_of.y, from)), first = cols.at(i) * kPage;
+    bool sees[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int t = lane + 32 * u, token = first + t;
+      sees[u] = is_far(v_exp, refs[((i - i0) * steps + t * steps / kPage) % n_refs]) && token <= pos &&
+                (a.window <= 0 || token > pos - a.window || token < a.n_first);
+    }
+    if (!__any_sync(0xffffffffu, sees[0] || sees[1]))
       continue;
-    const float *scale = a.cache.scale(page, head);
-    const int v_exp = exponent_field(scale[1]);
     const int8_t *block = a.cache.template block<D>(page, head);
-    const float factor = odd ? NAN : a.scale * kLog2e * scale[0], unit = two_to(v_exp - 127 - kSumBits);
+    float z[2][4] = {};
 #pragma unroll 1
-    for (int t0 = 0; t0 < kPage; t0 += 8) {
-      if (!is_far(v_exp, refs[((i - i0) * steps + t0 * steps / kPage) % n_refs]))
-        continue;
-      float z[8], top = -INFINITY;
+    for (int d = 0; d < D; d += 16) {
+      const uint4 k[2] = {ld_plain(block + lane * D + d), ld_plain(block + (lane + 32) * D + d)};
+      float x[4][4];
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const int token = cols.at(i) * kPage + t0 + u;
-        z[u] = -INFINITY;
-        if (token <= pos && (a.window <= 0 || token > pos - a.window || token < a.n_first)) {
-          float part[4] = {};
-#pragma unroll 1
-          for (int d = 0; d < D; d += 4) {
-            const char4 k = *reinterpret_cast<const char4 *>(block + (t0 + u) * D + d);
-            float x[4];
-            load4(q + d, a.q_vec, x);
+      for (int e = 0; e < 4; e++)
+        load4(q + d + 4 * e, a.q_vec, x[e]);
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              x[e] = at_least(at_most(x[e] * factor, kMostFactor), -kMostFactor);
-            part[0] = fmaf(x[0], k.x, part[0]), part[1] = fmaf(x[1], k.y, part[1]);
-            part[2] = fmaf(x[2], k.z, part[2]), part[3] = fmaf(x[3], k.w, part[3]);
-          }
-          z[u] = (part[0] + part[1]) + (part[2] + part[3]);
-        }
-        top = fmaxf(top, z[u]);
-      }
-      const float now = fmaxf(f.m, top), base = now > -INFINITY ? now : 0.0f, fade = fast_exp2(f.m - base);
-      float sum = 0.0f;
-#pragma unroll
-      for (int u = 0; u < 8; u++) {
-        z[u] = fast_exp2(z[u] - base);
-        sum += z[u];
-      }
-      f.m = now, f.l = fmaf(f.l, fade, sum);
-#pragma unroll
-      for (int n = 0; n < N; n += 4) {
-        float part[4] = {};
-#pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const char4 v = *reinterpret_cast<const char4 *>(block + (kPage + t0 + u) * D + d0 + n);
-          part[0] = fmaf(z[u], v.x, part[0]), part[1] = fmaf(z[u], v.y, part[1]);
-          part[2] = fmaf(z[u], v.z, part[2]), part[3] = fmaf(z[u], v.w, part[3]);
-        }
+      for (int u = 0; u < 2; u++) {
+        const uint32_t w[4] = {biased(k[u].x), biased(k[u].y), biased(k[u].z), biased(k[u].w)};
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          f.o[n + e] = fmaf(f.o[n + e], fade, part[e] * unit);
+#pragma unroll
+          for (int b = 0; b < 4; b++)
+            z[u][b] = fmaf(x[e][b] * lift, value(w[e], b), z[u][b]);
       }
     }
+    const float factor = at_least(at_most(row_factor * key_scale, kMostFactor), -kMostFactor);
+    float y[2], now = m, p[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      y[u] = sees[u] ? ((z[u][0] + z[u][1]) + (z[u][2] + z[u][3])) * factor : -INFINITY;
+      now = fmaxf(now, y[u]);
+    }
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1)
+      now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, x));
+    const float base = now > -INFINITY ? now : 0.0f, fade = fast_exp2(m - base), unit = two_to(v_exp - 127 - kSumBits);
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+      p[u] = sees[u] ? fast_exp2(y[u] - base) : 0.0f;
+    m = now, l = fmaf(l, fade, warp_sum(p[0] + p[1]));
+    float page_sum[N] = {};
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll 1
+      for (int t0 = 0; t0 < 32; t0 += 8) { // eight at a time, so that sums stay short
+        float part[N] = {};
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+          const int8_t *v = block + (kPage + 32 * u + t0 + t) * D + lane * N;
+          const uint32_t w = biased(N == 2 ? *reinterpret_cast<const uint16_t *>(v) : *reinterpret_cast<const uint32_t *>(v));
+          const float weight = __shfl_sync(0xffffffffu, p[u], t0 + t);
+#pragma unroll
+          for (int n = 0; n < N; n++)
+            part[n] = fmaf(weight, value(w, n), part[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++)
+          page_sum[n] += part[n];
+      }
+#pragma unroll
+    for (int n = 0; n < N; n++)
+      o[n] = fmaf(o[n], fade, page_sum[n] * unit);
   }
-  return f;
+  if (l == 0.0f) // a NaN passes, here and below
+    return;
+  const float2 near = *ml;
+  const float most = fmaxf(near.x, m), f = m > -INFINITY ? fast_exp2(m - most) : 1.0f;
+  const float near_sum = near.y != 0.0f ? near.y * fast_exp2(near.x - most) : 0.0f, sum = near_sum + l * f;
+#pragma unroll
+  for (int n = 0; n < N; n++)
+    mean[lane * N + n] = finite(fmaf(mean[lane * N + n], near_sum / sum, o[n] * (f / sum * (float)(1 << kSumBits))));
+  __syncwarp();
+  if (lane == 0)
+    *ml = make_float2(most, sum);
+  __syncwarp();
 }
 
 // Sequences of more than kMaxTokenRows rows (kv8_prompt.cu).

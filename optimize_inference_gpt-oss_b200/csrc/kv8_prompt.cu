@@ -170,8 +170,9 @@ template <typename QT, int D, int TILES> struct TileKernel {
                        kValueFull = kKeyFree + kKeyStages, kValueFree = kValueFull + kValueStages,
                        kRawFull = kValueFree + kValueStages, kRawFree = kRawFull + kRawStages, kDrained = kRawFree + kRawStages,
                        kBarCount = kDrained + 1;
-  static constexpr int kTmemAt = kBars + kBarCount * 8, kStopAt = kTmemAt + 4;
-  static constexpr int kSmem = kStopAt + 4 + 1024; // the base is brought to 1024 bytes, the swizzle's period
+  static constexpr int kTmemAt = kBars + kBarCount * 8, kStopAt = kTmemAt + 4, kFarAt = kStopAt + 4; // the second: far pages, their reference
+  static_assert(kRowsOfBlock * (D * 4 + 8) <= kMetaAt, "means of a block that has far pages");
+  static constexpr int kSmem = kFarAt + 8 + 1024; // the base is brought to 1024 bytes, the swizzle's period
   static_assert(kSmem <= 232448, "shared memory of a block");
 
   uint32_t base;
@@ -249,22 +250,73 @@ struct Parts {
   static size_t bytes(long blocks, int rows, int D) { return (size_t)blocks * rows * (D * 4 + 8); }
 };
 
+// The unit and the part of its columns that this block works on; false where there is nothing to do.  The last units of a
+// sequence, which see most, first.
+struct Work {
+  Unit u;
+  int split, col0, col1;
+  template <typename QT> __device__ __forceinline__ bool find(const Call<QT> &a, const Parts &parts, int rows) {
+    const int heads = a.cache.n_kv_heads, index = blockIdx.x / parts.splits;
+    split = blockIdx.x % parts.splits;
+    if (!u.find(a, (int)(gridDim.x / parts.splits / heads) - 1 - index / heads, index % heads, rows))
+      return false;
+    col0 = u.column(split, parts.splits), col1 = u.column(split + 1, parts.splits);
+    return col0 < col1;
+  }
+};
+
+// The end of a block that has met far pages, by its softmax warps: one per row adds them to the row's mean, which lies in
+// shared memory, and writes it.  What it needs is found again: nothing is held over the pages for its sake.
+template <typename QT, int D, int TILES> __device__ __noinline__ void finish_far(const Call<QT> &a, const Parts &parts, uint8_t *smem, int warps) {
+  using K = TileKernel<QT, D, TILES>;
+  constexpr int N = D / 32;
+  Work w = {};
+  (void)w.find(a, parts, K::kRowsOfBlock);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = (int)min(w.u.R - w.u.row0, (long)K::kRowsOfBlock);
+  const int *ref = reinterpret_cast<const int *>(smem + K::kFarAt) + 1;
+#pragma unroll 1
+  for (int r = warp; r < rows; r += warps) {
+    float *mean = reinterpret_cast<float *>(smem) + r * D;
+    float2 *ml = reinterpret_cast<float2 *>(smem + K::kRowsOfBlock * D * 4) + r;
+    const int token = (int)((w.u.row0 + r) / a.group), h = w.u.head * a.group + (int)((w.u.row0 + r) % a.group);
+    far_row<D>(a, w.u.s, w.u.head, w.u.cols, w.col0, w.col1, a.qkv + (size_t)(w.u.sp.row + token) * a.row_stride + (size_t)h * D,
+               w.u.sp.pos + token, ref, 1, 1, mean, ml);
+    const float2 x = *ml;
+    const size_t part = (size_t)blockIdx.x * K::kRowsOfBlock + r;
+    float f = x.y != 0.0f ? 1.0f : 0.0f; // a NaN passes
+    if (parts.splits > 1) {
+      if (lane == 0)
+        parts.ml[part] = x;
+    } else if (f != 0.0f) {
+      const float z = a.sinks ? sink_of(a, h) : -INFINITY, top = fmaxf(x.x, z), sum = x.y * (x.x > -INFINITY ? fast_exp2(x.x - top) : 1.0f);
+      f = sum / (sum + fast_exp2(z - top));
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const float v = f != 0.0f ? mean[lane * N + n] * f : 0.0f;
+      const size_t at = (size_t)(w.u.sp.row + token) * a.out_row_stride + (size_t)h * D + lane * N + n;
+      if (parts.splits > 1)
+        parts.o[part * D + lane * N + n] = v;
+      else if (a.out_f32)
+        static_cast<float *>(a.out)[at] = v;
+      else
+        store1(static_cast<uint16_t *>(a.out) + at, v);
+    }
+  }
+}
+
 template <typename QT, int D, int TILES>
-__global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __grid_constant__ Call<QT> a, Parts parts) {
+__global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __grid_constant__ Call<QT> a, const __grid_constant__ Parts parts) {
   using K = TileKernel<QT, D, TILES>;
   constexpr bool kSplit = K::kSplit;
   constexpr int kBuffers = K::kBuffers, kLeader = 32 * K::kConverters; // kLeader: the thread that asks for pages
   extern __shared__ uint8_t raw_smem[];
   pdl_prologue();
-  // the last units of a sequence, which see most, first
-  const int heads = a.cache.n_kv_heads, split = blockIdx.x % parts.splits, index = blockIdx.x / parts.splits;
-  Unit u = {};
-  if (!u.find(a, (int)(gridDim.x / parts.splits / heads) - 1 - index / heads, index % heads, K::kRowsOfBlock))
+  Work work = {};
+  if (!work.find(a, parts, K::kRowsOfBlock))
     return;
-  const int col0 = u.column(split, parts.splits), col1 = u.column(split + 1, parts.splits);
-  if (col0 == col1)
-    return;
-  const int s = u.s, head = u.head;
+  const Unit &u = work.u;
+  const int s = u.s, head = u.head, col0 = work.col0, col1 = work.col1;
   const Rows::Span sp = u.sp;
   const long R = u.R, row0 = u.row0;
   const Columns cols = u.cols;
@@ -276,6 +328,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
   k.stop = reinterpret_cast<volatile int *>(smem + K::kStopAt);
   k.giveups = a.giveups;
   Meta *const meta = reinterpret_cast<Meta *>(smem + K::kMetaAt);
+  volatile int *const far_block = reinterpret_cast<volatile int *>(smem + K::kFarAt); // 1: there are far pages; their reference
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31; // the same for all lanes, and known to be
   if (threadIdx.x == 0) {
     auto init = [&](int first, int n, int arrivals) {
@@ -293,7 +346,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
     init(K::kRawFull, K::kRawStages, 1);
     init(K::kRawFree, K::kRawStages, 4);
     init(K::kDrained, 1, 1);
-    *k.stop = 0;
+    *k.stop = 0, *far_block = 0;
     mbar_init_fence();
   }
   if (warp == K::kIssuer) {
@@ -508,47 +561,44 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
       if (ok) {
         tc_after_sync();
         const bool apart = parts.splits > 1;
-        const float z = !apart && a.sinks ? sink_of(a, h) : -INFINITY;
-        // What the tiles' sums and those of the row's far pages (maximum and sum there) are multiplied by; what a part leaves.
-        float f = 0.0f, f_far = 0.0f;
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        auto share = [&](float m_far, float l_far) {
-          if (l == 0.0f && l_far == 0.0f) // a NaN passes
-            return;
-          const float top = fmaxf(fmaxf(m, m_far), z);
-          const float fade = l != 0.0f ? (m > -INFINITY ? fast_exp2(m - top) : 1.0f) * two_to(-kTileBits) : 0.0f;
-          const float fade_far = l_far != 0.0f ? (m_far > -INFINITY ? fast_exp2(m_far - top) : 1.0f) : 0.0f;
-          const float seen = l * fade + l_far * fade_far, all = seen + fast_exp2(z - top);
-          f = fade * (float)(1 << (kNear - kValueBits)) / all, f_far = fade_far * (float)(1 << kSumBits) / all;
-          ml = make_float2(top, seen);
-        };
-        share(-INFINITY, 0.0f);
+        const float z = !apart && !far && a.sinks ? sink_of(a, h) : -INFINITY, unit = two_to(ref - 127);
+        float f = 0.0f;
+        if (l != 0.0f) { // a NaN passes
+          const float top = fmaxf(m, z), fade = (m > -INFINITY ? fast_exp2(m - top) : 1.0f) * two_to(-kTileBits);
+          f = fade * (float)(1 << (kNear - kValueBits)) / (l * fade + fast_exp2(z - top));
+        }
         const size_t part = (size_t)blockIdx.x * K::kRowsOfBlock + tile * kTile + r;
-        // Where the row goes; then 32 elements at a time through the warp's part of the queries' memory (all products
-        // are done), so that stores are of whole sectors.
-        const unsigned long long place =
-            !is ? ~0ull : apart ? part * D : (unsigned long long)(sp.row + token) * a.out_row_stride + (unsigned long long)h * D;
-        const uint32_t stage = k.base + K::kQueries + tile * (kSplit ? 2 : 1) * K::kQueryBytes + (warp & 3) * 4096;
-        auto write = [&](auto with_far) {
-          constexpr bool kFar = decltype(with_far)::value;
-          const float unit = two_to(ref - 127);
-          Unit v = {}; // for far pages, found again: nothing that only they need is held over the pages
-          if constexpr (kFar)
-            (void)v.find(a, (int)(gridDim.x / parts.splits / heads) - 1 - index / heads, index % heads, K::kRowsOfBlock);
+        if (apart && is)
+          parts.ml[part] = make_float2(m, l * two_to(-kTileBits));
+        if (far) { // means to shared memory (once no tile's products read there), for the whole block to go on from
+          for (int i = 0; i < tiles && ok && j > 0; i++)
+            ok = k.wait_warp(K::kOutDone + i, (j - 1) & 1);
+          if (ok) {
+            tc_after_sync();
+            float *mean = reinterpret_cast<float *>(smem) + (tile * kTile + r) * D;
+            reinterpret_cast<float2 *>(smem + K::kRowsOfBlock * D * 4)[tile * kTile + r] = make_float2(m, l * two_to(-kTileBits));
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              if (j > 0) {
+                tmem_load16(out_at(tile) + lanes + c, o);
+                tmem_loaded();
+              }
+#pragma unroll
+              for (int e = 0; e < 16; e++)
+                mean[c + e] = l != 0.0f ? finite(__uint_as_float(o[e]) * f * unit) : 0.0f;
+            }
+          }
+        } else {
+          // Where the row goes; then 32 elements at a time through the warp's part of the queries' memory (all products
+          // are done), so that stores are of whole sectors.
+          const unsigned long long place =
+              !is ? ~0ull : apart ? part * D : (unsigned long long)(sp.row + token) * a.out_row_stride + (unsigned long long)h * D;
+          const uint32_t stage = k.base + K::kQueries + tile * (kSplit ? 2 : 1) * K::kQueryBytes + (warp & 3) * 4096;
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
 #pragma unroll
             for (int half = 0; half < 32; half += 16) {
-              FarSum<16> fs = {};
-              if constexpr (kFar) {
-                if (is) {
-                  fs = far_pages<D, 16>(a, v.s, v.cols, v.column(split, parts.splits), v.column(split + 1, parts.splits), v.head,
-                                        a.qkv + (size_t)(sp.row + token) * a.row_stride + (size_t)h * D, pos, c + half,
-                                        &meta[j % kMeta].ref, 1, 1);
-                  share(fs.m, fs.l); // every time the same
-                }
-                __syncwarp();
-              }
               uint32_t o[16];
               if (j > 0) {
                 tmem_load16(out_at(tile) + lanes + c + half, o);
@@ -556,15 +606,11 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
               }
 #pragma unroll
               for (int e = 0; e < 16; e += 4) {
-                uint32_t v4[4];
+                uint32_t v[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                  float x = l != 0.0f ? __uint_as_float(o[e + i]) * f * unit : 0.0f;
-                  if constexpr (kFar)
-                    x = fmaf(fs.o[e + i], f_far, x);
-                  v4[i] = __float_as_uint(kFar && apart ? finite(x) : x); // a part's NaN shows by its sum
-                }
-                K::store16(stage + lane * 128 + (((half + e) / 4 ^ (lane & 7)) << 4), v4[0], v4[1], v4[2], v4[3]);
+                for (int i = 0; i < 4; i++)
+                  v[i] = l != 0.0f ? __float_as_uint(__uint_as_float(o[e + i]) * f * unit) : 0u;
+                K::store16(stage + lane * 128 + (((half + e) / 4 ^ (lane & 7)) << 4), v[0], v[1], v[2], v[3]);
               }
             }
             __syncwarp();
@@ -573,23 +619,21 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
               const int row_here = i * 4 + (lane >> 3), piece = lane & 7;
               const unsigned long long to = __shfl_sync(0xffffffffu, place, row_here) + c + piece * 4;
               const bool there = __shfl_sync(0xffffffffu, (int)is, row_here);
-              const uint4 w = lds16(stage + row_here * 128 + ((piece ^ (row_here & 7)) << 4));
-              const float4 w4 = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+              const uint4 v = lds16(stage + row_here * 128 + ((piece ^ (row_here & 7)) << 4));
+              const float4 v4 = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
               if (there && apart)
-                *reinterpret_cast<float4 *>(parts.o + to) = w4;
+                *reinterpret_cast<float4 *>(parts.o + to) = v4;
               else if (there)
-                store4(a, to, w4);
+                store4(a, to, v4);
             }
             __syncwarp();
           }
-        };
-        if (far)
-          write(std::true_type{});
-        else
-          write(std::false_type{});
-        if (apart && is)
-          parts.ml[part] = ml;
+        }
       }
+      // All softmax warps that have rows, also those that gave up; the others cannot take the call with the registers left.
+      asm volatile("bar.sync 1, %0;" ::"r"(128 * tiles) : "memory");
+      if (*far_block && !*k.stop)
+        finish_far<QT, D, TILES>(a, parts, smem, 4 * tiles);
     }
   } else if (warp < K::kIssuer) {
     // ---- codes to fp16: two warps the keys, two the values, a token per thread ----
@@ -597,7 +641,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
     const int t = threadIdx.x & 63;
     const bool values = warp >= K::kConverters + 2;
     const int *table = a.rows.pages + (size_t)s * a.rows.pages_stride;
-    int page_of = -1, held = col0 - 32, asked = 0, ref = 0; // ref: exponent of the first value scale there is
+    int page_of = -1, held = col0 - 32, asked = 0, ref = 0; // ref: exponent of the value scale that outputs are relative to
     bool any_far = false;
     unsigned there = 0; // of the columns held .. held + 31: those with a page, not a far one, that is still to be asked for
     float2 scale_of = make_float2(0.0f, 0.0f);
@@ -612,9 +656,8 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
         if (page_of >= 0)
           scale_of = *reinterpret_cast<const float2 *>(a.cache.scale(page_of, head));
         const int v_exp = page_of >= 0 ? exponent_field(scale_of.y) : 0;
-        const unsigned valued = __ballot_sync(0xffffffffu, v_exp != 0);
-        if (ref == 0 && valued)
-          ref = __shfl_sync(0xffffffffu, v_exp, __ffs(valued) - 1);
+        if (ref == 0)
+          ref = pick_ref(v_exp);
         const unsigned far = __ballot_sync(0xffffffffu, is_far(v_exp, ref));
         any_far = any_far || far;
         there = __ballot_sync(0xffffffffu, page_of >= 0) & ~far;
@@ -671,7 +714,9 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
           break;
         if (j >= K::kRawStages && !(ok = k.wait_warp((values ? K::kValueFree : K::kKeyFree) + stage, turn ^ 1)))
           break;
-        if (threadIdx.x == kLeader) // behind the last page all columns have been looked at
+        if (threadIdx.x == kLeader && !more && any_far) // behind the last page all columns have been looked at
+          far_block[0] = 1, far_block[1] = ref;
+        if (threadIdx.x == kLeader)
           meta[j % kMeta] = Meta{ring_token[stage], ring_scale[stage].x, ref, any_far};
         if (more) {
           if (!(ok = k.wait_warp(K::kRawFull + stage, turn)))
