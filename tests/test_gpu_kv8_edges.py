@@ -280,3 +280,60 @@ def test_entries_outside_the_pool_are_no_pages(gpu):
     assert pages[1, 0] == t.pages[0, 0] and pages[1, 1] == free[2] and refs[pages[1, 0]] == 2 and refs[free[2]] == 1
     assert t.d_len.get()[1] == 70
     assert all(not 0 <= p < 20 for p in pages[1, 2:])
+
+
+# ---- the four-tile form, where the others are tested at smaller sizes -------------------------------
+
+
+FILL = ([700, 430, 5, 64], [700, 430, 1, 0])  # rows for a block of four tiles on most SMs
+
+
+@pytest.mark.parametrize("out_name,pad,offset,pad_out", [("f32", 3, 1, 5), ("bf16", 8, 0, 8), ("f32", 4, 4, 4)])
+def test_four_tiles_strides_and_types(gpu, out_name, pad, offset, pad_out):
+    pkg = gpu
+    st = Step(pkg, 301 + pad, *FILL, 64, 8, 64, pkg.BF16, pad=pad, offset=offset, layers=2, layer=1, lead=2, trail=3).put()
+    st.check_attend(pkg.F32 if out_name == "f32" else pkg.BF16, pad_out=pad_out, sinks=st.r.standard_normal(64).astype(np.float32))
+
+
+def test_four_tiles_extreme_values(gpu):
+    """Scores far apart, equal scores, huge and tiny rows, pages of zeros and of scale 0, a negative and a zero scale; more
+    rows than max_new; windows that leave nothing where pages are missing."""
+    pkg = gpu
+    st = Step(pkg, 311, *FILL, 64, 8, 64, pkg.BF16, scales=(-24, 4), missing=[(0, 2, -1), (0, 3, 1 << 30), (1, 1, -9)])
+    st.x[:, :64] *= 40
+    st.x[:, 64:128] = 0
+    st.x[:, 128:192] *= np.float32(1e-18)
+    st.x[:, 192:256] *= np.float32(2e4)
+    st.x = widen(pkg, st.x, pkg.BF16)
+    st.scales[0, st.pages[0, 5], :, 1] = 0
+    st.scales[0, st.pages[0, 4], :, 0] = 0
+    st.scales[0, st.pages[0, 6], :, 1] = 2.0 ** -100
+    st.codes[0, st.pages[1, 0]] = 0
+    st.put()
+    st.check_attend(scale=-0.25)
+    st.check_attend(scale=0.0, sinks=np.full(64, -1e30, np.float32))
+    st.check_attend(window=30, max_new=640)
+    assert pkg.load().gptoss_wait_giveups() == 0
+
+
+# ---- release and attention together --------------------------------------------------------------
+
+
+@pytest.mark.parametrize("window,first", [(1, 0), (64, 0), (65, 64), (128, 4), (100, 70), (1000, 0)])
+@pytest.mark.parametrize("new", [1, 9])
+def test_what_is_released_is_not_missed(gpu, window, first, new):
+    """Pages let go of behind a window belong to others from then on (junk, scales that are NaN): the rows that come
+    next give what the definition gives with the whole cache."""
+    pkg = gpu
+    lens = [1, 64, 65, 300, 383, 256]
+    st = Step(pkg, 321 + window, [n + new for n in lens], [new] * 6, 8, 2, 64, pkg.BF16).put()
+    ref = want(st, window=window, first=first)
+    refs = np.bincount(st.pages[st.pages >= 0], minlength=st.codes.shape[1]).astype(np.int32)
+    d_len, d_refs, d_pages = (st.dev.put_inout(a) for a in (np.asarray(lens, np.int32), refs, st.pages))
+    pkg.kv8_release(6, st.dev.put(np.arange(6, dtype=np.int32)), 6, d_len, d_pages, st.width, len(refs), d_refs, window, first)
+    left = d_refs.get()
+    assert (left <= refs).all() and (left < refs).any() == (window < 1000)
+    st.scales[:, (refs > 0) & (left == 0)] = np.nan
+    st.d_scales, st.d_pages = st.dev.put_inout(st.scales), d_pages
+    st.pool = pkg.kv8_pool(st.d_codes, st.d_scales, 1, st.codes.shape[1], st.heads, st.D)
+    check(st, run(st, pkg.F32, window=window, first=first), *ref, pkg.F32)
