@@ -15,8 +15,8 @@
 //   - codes become fp16 exactly (kv8_mma.cuh); key scales multiply the scores, value scales, powers
 //     of two, multiply the codes relative to a reference of the warp (kv8_attention.cuh, also on pages far from it);
 //   - queries are brought to fp16 range by a power of two per row; a bf16 row is then exact, an fp32 row
-//     is two fp16 parts and two products, and so are its softmax weights, which is what keeps fp32's
-//     accuracy on these tensor cores;
+//     is two fp16 parts and two products, and so are its softmax weights, and its sums are folded (kFold), which is what
+//     keeps fp32's accuracy on these tensor cores;
 //   - the weights carry a factor 2^9, so that weights down to 2^-23 of the largest are normal fp16;
 //   - work is cut into equal pieces of pages over all blocks whatever the lengths (a long sequence
 //     beside short ones, one sequence alone); a sequence cut across blocks is joined by merge_pieces.
@@ -74,6 +74,8 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
   static constexpr int kResult = kRows * (kPitch * 4 + 8); // a warp's results, which lie where its ring was
   static constexpr int kRing = 2 * kDepth * kPart > kResult ? 2 * kDepth * kPart : kResult; // 8 or 16 KB per warp
   static constexpr int kSmem = kTokenWarps * (kRing + 2 * kDepth * 8 + kDepth * 16 + 4);
+  static constexpr bool kFolds = kSplit && !WHOLE;
+  static constexpr int kFoldSteps = kFold / (2 * TT), kFolded = kFolds ? (4 * DT + 2) * RB : 1;
   using VWord = typename std::conditional<D == 64, uint2, uint4>::type;
 
   uint32_t q[RB][KS][2], q_rest[kSplit ? RB : 1][kSplit ? KS : 1][2];
@@ -84,6 +86,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
   uint32_t ring, bars; // this warp's, as shared-space addresses
   int4 *slots;         // what a part is: page, step, scales
   int done;            // parts used so far, over all items
+  int since;           // steps since outputs were last folded; negative: they never were
   bool lost;           // a copy did not arrive in time
 
   __device__ __forceinline__ void setup() {
@@ -151,7 +154,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
   }
 
   __device__ __forceinline__ void begin() {
-    ref = 0, met_far = false;
+    ref = 0, met_far = false, since = -kFoldSteps;
 #pragma unroll
     for (int b = 0; b < RB; b++)
 #pragma unroll
@@ -160,6 +163,29 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
 #pragma unroll
         for (int j = 0; j < DT; j++)
           o[b][j][e] = o[b][j][2 + e] = 0.0f;
+      }
+  }
+
+  // Outputs so far to (or, at the end, from) this thread's memory, where they are relative to the rows' maxima of then.
+  template <bool BACK> __device__ __forceinline__ void fold(volatile float (&kept)[kFolded], bool first) {
+#pragma unroll
+    for (int b = 0; b < RB; b++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        volatile float *at = kept + (2 * b + e) * (2 * DT + 1);
+        const float then = first ? -INFINITY : at[2 * DT], f = then > -INFINITY ? fast_exp2(then - m[b][e]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < DT; j++)
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            float &x = o[b][j][2 * half + e];
+            const float sum = first ? x : fmaf(at[2 * j + half], f, x);
+            if (!BACK)
+              at[2 * j + half] = sum;
+            x = BACK ? sum : 0.0f;
+          }
+        if (!BACK)
+          at[2 * DT] = m[b][e];
       }
   }
 
@@ -312,7 +338,7 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
 
   // The columns [i0, i1) of an item, steps dealt to the block's warps in turn.
   __device__ __forceinline__ void run(const Call<QT> &a, const Rows::Span &sp, int s, int head, int row0, const Columns &cols,
-                                      int i0, int i1, int min_pos, int max_pos) {
+                                      int i0, int i1, int min_pos, int max_pos, volatile float (&kept)[kFolded]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int j0 = i0 * kSteps + warp, end = i1 * kSteps;
     const int steps = j0 < end && !lost ? (end - j0 + kTokenWarps - 1) / kTokenWarps : 0;
@@ -396,6 +422,9 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
         break;
       }
       add_values(w, v_exp, part_at(done, 1));
+      if constexpr (kFolds)
+        if (++since == 0 || since == kFoldSteps)
+          fold<false>(kept, since == 0), since = 0;
       __syncwarp();
       ask_values(done + kDepth);
     }
@@ -406,6 +435,9 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
         arrived(p, 0), arrived(p, 1);
       done = asked;
     }
+    if constexpr (kFolds)
+      if (since >= 0)
+        fold<true>(kept, false);
   }
 
   // The warps' results, and the far pages of columns [i0, i1), joined: into the output, or into a piece for
@@ -488,7 +520,8 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
 
   __device__ __forceinline__ void item(const Call<QT> &a, const Rows::Span &sp, int s, int head, int rg, const Columns &cols,
                                        int i0, int i1, int min_pos, int max_pos, float *piece_o, float2 *piece_ml) {
-    run(a, sp, s, head, rg * kRows, cols, i0, i1, min_pos, max_pos);
+    volatile float kept[kFolded]; // volatile: in memory, the registers are full
+    run(a, sp, s, head, rg * kRows, cols, i0, i1, min_pos, max_pos, kept);
     finish(a, sp, s, head, rg * kRows, cols, i0, i1, piece_o, piece_ml);
   }
 };

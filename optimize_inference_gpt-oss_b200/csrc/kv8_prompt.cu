@@ -147,6 +147,7 @@ __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.s
 
 template <typename QT, int D, int TILES> struct TileKernel {
   static constexpr bool kSplit = sizeof(QT) == 4;
+  static constexpr int kFoldPages = kSplit ? kFold / (2 * kPage / 16) : 1 << 30; // products of this page start O afresh
   static constexpr int kBuffers = TILES == 2 ? 2 : 1;                  // of scores, per tile
   static constexpr int kConverters = 4 * TILES, kIssuer = kConverters + 4, kThreads = 32 * (kIssuer + 1);
   static constexpr int kRowsOfBlock = kTile * TILES;
@@ -436,6 +437,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
         arrive_warp(k.bar(K::kQueryFull));
       }
       float m = -INFINITY, l = 0.0f;
+      float kept[kSplit ? D : 1], m_kept = -INFINITY; // O of the pages before the last fold, relative to the maximum of then
       int j = 0, ref = 0;
       bool far = false;
       // What this thread's row does not see of a page gets a score below all others.  Only pages at the edge of
@@ -485,14 +487,16 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
         // A factor that is not 0, so that what is masked stays below; 2^-100 of a score is as good as 0.
         const float f = any ? at_least(at_most(row_factor * it.key_scale, kMostFactor), 0x1p-100f) : 1.0f;
         const float now = any ? fmaxf(m, top * f) : m;
-        if (__any_sync(0xffffffffu, now > m + kRise)) {
-          const float fade = now > -INFINITY ? fast_exp2(m - now) : 1.0f;
-          m = now;
+        const bool moved = __any_sync(0xffffffffu, now > m + kRise), fold = kSplit && j > 0 && j % K::kFoldPages == 0;
+        if (moved || fold) {
+          const float fade = moved && now > -INFINITY ? fast_exp2(m - now) : 1.0f;
+          m = moved ? now : m;
           l *= fade;
           if (j > 0) {
             if (!k.wait_warp(K::kOutDone + tile, (j - 1) & 1))
               return false;
             tc_after_sync();
+            const float then = m_kept > -INFINITY ? fast_exp2(m_kept - m) : 0.0f;
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
@@ -501,8 +505,16 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
 #pragma unroll
               for (int e = 0; e < 16; e++)
                 o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+              if constexpr (kSplit)
+                if (fold) {
+#pragma unroll
+                  for (int e = 0; e < 16; e++)
+                    kept[c + e] = j == K::kFoldPages ? __uint_as_float(o[e]) : fmaf(kept[c + e], then, __uint_as_float(o[e]));
+                  continue; // the next product overwrites O
+                }
               tmem_store16(out_at(tile) + lanes + c, o);
             }
+            m_kept = fold ? m : m_kept;
           }
         }
         const float off = (float)kTileBits - (m > -INFINITY ? m : 0.0f);
@@ -561,6 +573,20 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
       if (ok) {
         tc_after_sync();
         const bool apart = parts.splits > 1;
+        // 16 elements of O from c on, those folded before included.
+        auto load_out = [&](int c, uint32_t (&o)[16]) {
+          if (j > 0) {
+            tmem_load16(out_at(tile) + lanes + c, o);
+            tmem_loaded();
+          }
+          if constexpr (kSplit)
+            if (j > K::kFoldPages) {
+              const float then = m_kept > -INFINITY ? fast_exp2(m_kept - m) : 0.0f;
+#pragma unroll
+              for (int e = 0; e < 16; e++)
+                o[e] = __float_as_uint(fmaf(kept[c + e], then, __uint_as_float(o[e])));
+            }
+        };
         const float z = !apart && !far && a.sinks ? sink_of(a, h) : -INFINITY, unit = two_to(ref - 127);
         float f = 0.0f;
         if (l != 0.0f) { // a NaN passes
@@ -580,10 +606,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
-              if (j > 0) {
-                tmem_load16(out_at(tile) + lanes + c, o);
-                tmem_loaded();
-              }
+              load_out(c, o);
 #pragma unroll
               for (int e = 0; e < 16; e++)
                 mean[c + e] = l != 0.0f ? finite(__uint_as_float(o[e]) * f * unit) : 0.0f;
@@ -600,10 +623,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
 #pragma unroll
             for (int half = 0; half < 32; half += 16) {
               uint32_t o[16];
-              if (j > 0) {
-                tmem_load16(out_at(tile) + lanes + c + half, o);
-                tmem_loaded();
-              }
+              load_out(c + half, o);
 #pragma unroll
               for (int e = 0; e < 16; e += 4) {
                 uint32_t v[4];
@@ -797,7 +817,7 @@ __global__ void __launch_bounds__(32 * (4 * TILES + 5), 1) attend_tiles(const __
         const uint32_t values = values0 + value_stage * (K::kPageBytes / 16);
 #pragma unroll
         for (int part = 0; part < (kSplit ? 2 : 1); part++)
-          mma4_tmem<TILES == 2 ? 16 : 32>(out_at(tile), scores_at(tile, j) + part * 32, values, kOutShape, j + part > 0);
+          mma4_tmem<TILES == 2 ? 16 : 32>(out_at(tile), scores_at(tile, j) + part * 32, values, kOutShape, j % K::kFoldPages + part > 0);
         tc_commit(k.bar(K::kOutDone + tile));
         if (tile == tiles - 1)
           tc_commit(k.bar(K::kValueFree + value_stage));

@@ -337,3 +337,34 @@ def test_what_is_released_is_not_missed(gpu, window, first, new):
     st.d_scales, st.d_pages = st.dev.put_inout(st.scales), d_pages
     st.pool = pkg.kv8_pool(st.d_codes, st.d_scales, 1, st.codes.shape[1], st.heads, st.D)
     check(st, run(st, pkg.F32, window=window, first=first), *ref, pkg.F32)
+
+
+# ---- long sums ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,new,kv,n_q,heads", [(1, 5000, 5000, 4, 1), (296, 1, 9600, 16, 4), (150, 3, 9600, 16, 4), (1, 30, 40000, 4, 1)])
+def test_fp32_rows_over_long_contexts(gpu, n, new, kv, n_q, heads):
+    """The matrix units cut off, on average half a unit (2^-24) per addition, and sums that grow evenly lose half of what
+    their last additions would: over 64 additions 64 / 2 * 2^-24 = 2^-19 of the whole, to which everything else that
+    rounds to nearest adds little.  One chain of additions over all tokens loses 10 to 100 times that.  Values of one
+    sign, so that nothing cancels."""
+    pkg = gpu
+    st = Step(pkg, 401 + new, [kv], [n * new], n_q, heads, 64, pkg.F32)
+    st.row_start, st.kv_len = np.arange(0, n * new + 1, new, dtype=np.int32), np.full(n, kv, np.int32)
+    st.pages, st.max_new = np.tile(st.pages, (n, 1)), new  # all read one sequence's pages
+    st.x[:, :n_q * 64] *= 0.25
+    st.codes[0, :, :, 1] = np.abs(st.codes[0, :, :, 1])
+    st.put()
+    got = run(st, pkg.F32).astype(np.float64)
+    rows = np.unique(np.linspace(0, st.T - 1, 24).astype(int))  # the definition at some of the rows
+    k, v = ((st.codes[0, st.pages[0], :, i].astype(np.float64) * st.scales[0, st.pages[0], :, i][..., None, None])
+            .transpose(1, 0, 2, 3).reshape(heads, -1, 64) for i in (0, 1))
+    ref = np.zeros((len(rows), n_q, 64))
+    for i, r in enumerate(rows):
+        pos = kv - new + r % new
+        q = st.x[r, :n_q * 64].reshape(n_q, 64).astype(np.float64)
+        for h in range(n_q):
+            z = 0.125 * (k[h * heads // n_q, :pos + 1] @ q[h])
+            w = np.exp(z - z.max())
+            ref[i, h] = w @ v[h * heads // n_q, :pos + 1] / w.sum()
+    assert np.linalg.norm(got[rows] - ref) <= 2.0 ** -19 * np.linalg.norm(ref)
