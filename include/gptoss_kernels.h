@@ -395,7 +395,8 @@ GPTOSS_API int gptoss_argmax_noalloc(gptoss_stream_t stream, int T, const void *
  * The reference has none of this (its cache has fixed slots per request, keys in bf16 and one
  * scale per value vector, gptoss_kv_cache_write above).  A page holds 64 tokens.  For each page,
  * key/value head and kind (0 key, 1 value) it has 64 x head_dim int8 codes and one fp32 scale
- * that is a power of two; a value is code * scale, which is exact in bf16 and fp32.
+ * that is a power of two; a value is code * scale, which is exact in bf16 and fp32 (but for what append
+ * makes of an infinity, 64 * 2^122 = 2^128).
  *
  * A sequence's token at position p lives in slot p % 64 of the page pages[s * pages_stride + p / 64]
  * of its page table row; -1, or any number outside [0, n_pages), means that there is no page.  One
@@ -431,7 +432,7 @@ typedef struct {
  * of two keep every step of this exact except the one rounding, and bound what repeated growth
  * can cost: each regrowth at least doubles the scale, so all earlier roundings together stay below
  * one step of the final scale.  A page whose slot 0 is written starts afresh, whatever it held.
- * NaN is stored as 0, infinities as the largest finite fp32.  Rows whose position has no page are
+ * NaN is stored as 0, infinities as the largest finite fp32 (whose code rounds up to 64 * 2^122).  Rows whose position has no page are
  * skipped; slots behind the last row are left as they were.
  */
 GPTOSS_API int gptoss_kv8_append(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int layer, int T,
@@ -453,11 +454,14 @@ GPTOSS_API int gptoss_kv8_append(gptoss_stream_t stream, const gptoss_kv8_pool_t
  * sequence are left as they were.
  * Products are taken on the tensor cores with the codes as they are (exact in fp16); fp32 rows
  * (qkv_dtype GPTOSS_F32) and the softmax weights that go with them are carried as two fp16 parts, so
- * that the result has fp32's accuracy; the weights of bf16 rows are rounded to one fp16 number (2^-11),
- * whatever the output's type; a weight below 2^-33 of the row's largest may count as 0; sums are fp32.
+ * that the result has fp32's accuracy (1e-6 relative at contexts of thousands of tokens); the weights of
+ * bf16 rows are rounded to one fp16 number (2^-11), whatever the output's type; a weight below 2^-33 of the
+ * row's largest may count as 0; sums are fp32.
  * Pages whose value scale is more than 2^10 from that of the others are summed apart, in fp32, and
  * joined (slower: made for pages that hardly ever are), so that a row's result does not depend on the size
  * of values it does not see.  Scores z have to lie within fp32's range.
+ * A wait inside a kernel that runs out (half a second; none should) is counted by gptoss_wait_giveups();
+ * the call has returned GPTOSS_OK by then, and rows of the block concerned are incomplete or not written.
  * workspace: gptoss_kv8_attention_workspace bytes (for the same arguments on the same device),
  * 16-byte aligned, contents irrelevant; calls that may overlap in time need one each.
  */
@@ -506,9 +510,9 @@ GPTOSS_API int gptoss_kv8_reserve(gptoss_stream_t stream, int n, const int *seqs
 /*
  * Makes children[i] a copy of parents[i]: its full pages are shared (refs + 1), a last page that is
  * not full is copied, in every layer, into a free page of its own.  Pages a parent reserved ahead
- * are not taken over.  Not served: a child that is not empty (kv_len 0, no pages), that was listed
- * before or that is a parent in the same call, a parent whose kv_len is outside the table, or no free page left.  A parent may be
- * listed any number of times.
+ * are not taken over.  Not served: a child that is not empty (kv_len 0, no pages) or that was listed
+ * before, a parent that is named as a child anywhere in the same call or whose kv_len is outside the
+ * table, or no free page left.  A parent may be listed any number of times; n is at most n_seqs.
  */
 GPTOSS_API int gptoss_kv8_fork(gptoss_stream_t stream, const gptoss_kv8_pool_t *pool, int n,
                                const int *parents, const int *children, int n_seqs, int *kv_len,

@@ -22,7 +22,7 @@ namespace gptoss {
 namespace kv8 {
 namespace {
 
-// |x| of a value to be stored: a NaN counts as 0, an infinity as the largest finite value.
+// A value as it is stored: a NaN as 0, an infinity as the largest finite value.
 __device__ __forceinline__ float storable(float x) {
   return x != x ? 0.0f : fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f);
 }

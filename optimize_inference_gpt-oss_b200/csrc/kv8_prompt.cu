@@ -10,18 +10,21 @@
 // What would bound it at D = 64 is the exponential (16 per clock and SM: 512 clocks for a 128 x 64 tile against some
 // 320 of matrix instructions); what does is how far the steps of a tile, which wait for each other (scores,
 // weights, product), are covered by those of the others: 810 clocks per tile and page with four tiles, 1230 with two.
-// An 8192-token prompt of 64 heads takes 0.79 ms, 0.70 PFLOP/s.  So:
+// An 8192-token prompt of 64 heads takes 0.78 ms, 0.70 PFLOP/s.  (Two tiles keep all they need in registers; four, at 80,
+// do not: -Xptxas -v shows 108 bytes of spill stores and 216 of loads per thread.)  So:
 //   - four warps per tile: softmax.  A row's running maximum is raised only when the new one is 2^8 above it, so
 //     that O is rescaled a few times per row and not once per page;
 //   - four warps: codes (brought by the copy engine into a ring of raw pages) to fp16 in the 128-byte swizzled
-//     form the matrix instruction reads, once for both tiles; two warps for the keys and two for the values, since
+//     form the matrix instruction reads, once for all tiles; two warps for the keys and two for the values, since
 //     what a page costs them is mostly waiting (barriers, the fence before the matrix unit may read);
 //   - one warp: one of its threads issues the matrix instructions.  With two tiles scores have two buffers each, so
 //     that the next page's are ready when a softmax warp comes for them; with four there is room for one;
 //   - where there are few units (a chunk of some rows against a long context) their columns are shared out over more
 //     blocks and joined by merge_parts.
 // Queries, codes and weights are represented as in kv8_attention.cu: fp16, exact for codes and bf16 rows; fp32 rows
-// and their weights in two parts with two products.
+// and their weights in two parts with two products, and O folded into the softmax threads' memory every kFoldPages pages.
+// Value scales are relative to one reference per block; far pages (kv8_attention.cuh) are left out of the loop and
+// added by finish_far.
 // Every wait is bounded: one that runs out is counted, tells the block's other roles, and the block frees its
 // tensor memory and ends.
 #include <algorithm>
@@ -910,8 +913,8 @@ template <typename QT> void launch_tiles(cudaStream_t stream, const Call<QT> &a,
     return;
   }
   // Four tiles fit tensor memory at 64 elements and bf16 rows (one part of weights).  Where they would leave SMs
-  // without a block, two: one prompt, 64 and 8 heads, two tiles against four: 700 tokens (84 blocks of four) 27 / 32 us,
-  // 1000 (124) 37 / 39, 1300 (160) 58 / 50, 4000 (504) 291 / 221; five chunks (133) 167 / 132.
+  // without a block, two: one prompt, 64 and 8 heads, two tiles against four: 700 tokens (80 by the condition below)
+  // 27 / 32 us, 1000 (120) 37 / 39, 1300 (160) 58 / 50, 4000 (496) 291 / 221; five chunks (144) 167 / 132.
   if constexpr (sizeof(QT) == 2)
     if ((four - a.rows.n_seqs) * a.cache.n_kv_heads >= sm_count() * 7 / 8) {
       launch_with<QT, 64, 4>(stream, a, four, 1, workspace);
