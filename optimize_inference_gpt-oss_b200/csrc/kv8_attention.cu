@@ -336,7 +336,11 @@ template <typename QT, int D, int RB, bool WHOLE> struct TokenKernel {
                  "l"(block + (size_t)(kind * kPage + step * CH) * D), "r"(kPart), "r"(bar)
                  : "memory");
   }
-  __device__ __forceinline__ bool arrived(int p, int kind) const { return mbar_wait_at(bar_at(p, kind), p / kDepth & 1); }
+  // One answer for the warp: where the wait runs out, lanes that had seen the barrier complete must not go on alone to
+  // what the whole warp does next.
+  __device__ __forceinline__ bool arrived(int p, int kind) const {
+    return __all_sync(0xffffffffu, mbar_wait_at(bar_at(p, kind), p / kDepth & 1));
+  }
 
   // The columns [i0, i1) of an item, steps dealt to the block's warps in turn.
   __device__ __forceinline__ void run(const Call<QT> &a, const Rows::Span &sp, int s, int head, int row0, const Columns &cols,
