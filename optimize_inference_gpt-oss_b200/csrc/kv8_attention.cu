@@ -20,8 +20,8 @@
 //   - the weights carry a factor 2^9, so that weights down to 2^-23 of the largest are normal fp16;
 //   - work is cut into equal pieces of pages over all blocks whatever the lengths (a long sequence
 //     beside short ones, one sequence alone); a sequence cut across blocks is joined by merge_pieces.
-// Measured: 64 sequences, 8000 tokens on average, 8 heads of 64: 0.57 GB in 105 us with the join, 0.82 of a copy's
-// rate.  One sequence of 131072 tokens, heads of 128: 0.27 GB in 67 us, of which 3 us finding the pieces, 5 us
+// Measured: 64 sequences, 8000 tokens on average, 8 heads of 64: 0.57 GB in 107 us with the join, 0.81 of a copy's
+// rate.  One sequence of 131072 tokens, heads of 128: 0.27 GB in 68 us, of which 3 us finding the pieces, 5 us
 // joining.  Some 700 instructions per page and warp at 2 per clock and SM: the next bound is issue, not memory.
 // Most forms for 32 rows, fp32 rows or 128-wide heads need more registers than there are and spill (-Xptxas -v: up to
 // 200 bytes of stores per thread for bf16 rows, 830 for 32 fp32 rows of 128).
